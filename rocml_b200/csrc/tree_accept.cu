@@ -1,0 +1,139 @@
+// Which drafted nodes a sampler's tokens confirm, and their keys and values moved behind the context.
+//
+// Node i is like its parent's draw when token[i] == sampled[parent[i]] and no earlier child of that parent has the same token; node
+// 0 always is.  It is confirmed when it and all its ancestors are: with the rows of bits that the attention reads
+// (ancestors and the node itself) that is (visible_i & ~like) == 0, without a walk from node to node.  The confirmed nodes form one
+// path, and a node's place on it is its depth, popcount(visible_i) - 1.
+//
+// Their keys and values lie at places c + node and belong at c + depth.  A thread owns 16 bytes of one head of one layer for the whole
+// path.  Nodes come after their parents, so depth <= node: writing place c + d destroys nothing that a deeper node is still read
+// from (its node is larger than d), and a batch of loads ahead of its stores is in order.  Eight loads are in flight a thread; the
+// path's rows once in and once out bound the kernel.  Every block of a sequence finds the path again (microseconds less than
+// a launch of its own would take); the first writes it down.
+#include "common.cuh"
+#include "api.h"
+
+namespace {
+constexpr int MAX_NODES = 256, WORDS = MAX_NODES / 32, THREADS = 256, BATCH = 8;
+
+template <typename Vec>
+__global__ void __launch_bounds__(THREADS)
+tree_accept_kernel(const int* __restrict__ tokens, const int* __restrict__ parents, const int* __restrict__ visible, int words,
+                   const int* __restrict__ sampled, const int* __restrict__ cu_q, int* __restrict__ path, int path_ld,
+                   int* __restrict__ counts, int* __restrict__ next_token, const int* __restrict__ seq_slot, const int* __restrict__ kv_len,
+                   const int* __restrict__ block_table, int max_pages, Vec* k, Vec* v, int units, int nkv, long long n_pages,
+                   int vecs) {
+    rb::pdl_trigger();
+    rb::pdl_wait();
+    __shared__ int first[MAX_NODES], way[MAX_NODES];
+    __shared__ unsigned int like_bits[WORDS];
+    __shared__ int count;
+    const int b = blockIdx.y, tid = threadIdx.x;
+    const int slot = seq_slot ? seq_slot[b] : 0, q0 = cu_q[b];
+    const int n = min(min(cu_q[b + 1] - q0, words * 32), path_ld);
+    if (slot < 0 || n <= 0) return;
+    first[tid] = MAX_NODES;
+    way[tid] = -1;
+    if (tid == 0) count = 0;
+    __syncthreads();
+    int up = -1;
+    bool like = false;
+    if (tid < n) {
+        up = parents[q0 + tid];
+        like = up >= 0 && up < tid && tokens[q0 + tid] == sampled[q0 + up];
+        if (like) atomicMin(&first[up], tid);
+    }
+    __syncthreads();
+    like = tid < n && (tid == 0 || (like && first[up] == tid));
+    const unsigned int ballot = __ballot_sync(0xffffffffu, like);
+    if ((tid & 31) == 0) like_bits[tid >> 5] = ballot;
+    __syncthreads();
+    if (tid < n) {
+        bool kept = like;
+        int depth = -1;
+        for (int w = 0; w * 32 < n; ++w) {
+            unsigned int bits = (unsigned int)visible[(size_t)(q0 + tid) * words + w];
+            if (n - w * 32 < 32) bits &= (1u << (n - w * 32)) - 1u;
+            kept = kept && (bits & ~like_bits[w]) == 0;
+            depth += __popc(bits);
+        }
+        if (kept && depth >= 0 && depth <= tid) {
+            way[depth] = tid;
+            atomicAdd(&count, 1);
+        }
+    }
+    __syncthreads();
+    const int n_path = count;
+    if (blockIdx.x == 0) {
+        for (int i = tid; i < path_ld; i += THREADS) path[(size_t)b * path_ld + i] = i < n_path ? way[i] : -1;
+        if (tid == 0) {
+            counts[b] = n_path;
+            next_token[b] = n_path > 0 && way[n_path - 1] >= 0 ? sampled[q0 + way[n_path - 1]] : -1;
+        }
+    }
+    if (!k) return;
+    const int len = kv_len[b], ctx = len - (cu_q[b + 1] - q0);
+    if (ctx < 0 || len > max_pages * RB_PAGE) return;
+    // this thread's 16 bytes: unit (keys or values, layer, head) and place inside the head's row
+    const long long at = (long long)blockIdx.x * THREADS + tid;
+    const int unit = (int)(at / vecs), col = (int)(at % vecs);
+    if (unit >= 2 * units) return;
+    Vec* cache = unit < units ? k : v;
+    const int lh = unit < units ? unit : unit - units, layer = lh / nkv, head = lh % nkv;
+    const int* table = block_table + (size_t)slot * max_pages;
+    auto row = [&](int place) -> Vec* {
+        const int page = table[place / RB_PAGE];
+        if (page < 0) return nullptr;
+        return cache + ((((size_t)layer * n_pages + page) * nkv + head) * RB_PAGE + place % RB_PAGE) * vecs + col;
+    };
+    for (int d0 = 0; d0 < n_path; d0 += BATCH) {
+        Vec x[BATCH];
+        Vec* to[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int d = d0 + i, node = d < n_path ? way[d] : -1;
+            to[i] = nullptr;
+            if (node > d) {                          // (a node that is where it belongs stays)
+                const Vec* from = row(ctx + node);
+                to[i] = from ? row(ctx + d) : nullptr;
+                if (to[i]) x[i] = *from;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+            if (to[i]) *to[i] = x[i];
+    }
+}
+
+template <typename Vec>
+int launch_accept(const int* tokens, const int* parents, const int* visible, int words, const int* sampled, const int* cu_q, int n_seqs,
+                  int* path, int path_ld, int* counts, int* next_token, const int* seq_slot, const int* kv_len, const int* block_table,
+                  int max_pages, void* k, void* v, int layers, int nkv, long long n_pages, int row_bytes, cudaStream_t stream) {
+    const int vecs = row_bytes / (int)sizeof(Vec);
+    const long long threads = k ? 2ll * layers * nkv * vecs : 1;
+    const long long blocks = (threads + THREADS - 1) / THREADS;
+    if (blocks > 0x7fffffffll) return RB_ERR_BAD_SIZE;
+    RB_LAUNCH((tree_accept_kernel<Vec>), dim3((unsigned)blocks, n_seqs), dim3(THREADS), 0, stream, tokens, parents, visible, words, sampled, cu_q,
+              path, path_ld, counts, next_token, seq_slot, kv_len, block_table, max_pages, (Vec*)k, (Vec*)v, layers * nkv, nkv, n_pages, vecs);
+    return RB_OK;
+}
+}  // namespace
+
+// k, v: [layers, n_pages, nkv, 64, row_bytes], or null (nothing is moved).
+extern "C" int rb_tree_accept(const int* tokens, const int* parents, const int* visible, int words, const int* sampled, const int* cu_q,
+                              int n_seqs, int* path, int path_ld, int* counts, int* next_token, const int* seq_slot, const int* kv_len,
+                              const int* block_table, int max_pages, void* k, void* v, int layers, int nkv, long long n_pages,
+                              int row_bytes, int element_bytes, void* stream) {
+    if (n_seqs <= 0) return RB_OK;
+    if (words <= 0 || words > WORDS || path_ld <= 0 || path_ld > MAX_NODES || n_seqs > 65535) return RB_ERR_BAD_SIZE;
+    if ((k == nullptr) != (v == nullptr)) return RB_ERR_BAD_SIZE;
+    if (k && (!seq_slot || !kv_len || !block_table || layers <= 0 || nkv <= 0 || row_bytes <= 0 || max_pages <= 0)) return RB_ERR_BAD_SIZE;
+    cudaStream_t st = (cudaStream_t)stream;
+#define RB_ACCEPT_ARGS tokens, parents, visible, words, sampled, cu_q, n_seqs, path, path_ld, counts, next_token, seq_slot, kv_len, block_table, \
+                       max_pages, k, v, layers, nkv, n_pages, row_bytes, st
+    if (!k || (row_bytes % 16 == 0 && !(((uintptr_t)k | (uintptr_t)v) & 15))) return launch_accept<uint4>(RB_ACCEPT_ARGS);
+    if (element_bytes == 4 && row_bytes % 4 == 0) return launch_accept<uint32_t>(RB_ACCEPT_ARGS);
+    if (element_bytes == 2 && row_bytes % 2 == 0) return launch_accept<uint16_t>(RB_ACCEPT_ARGS);
+    return RB_ERR_BAD_DTYPE;
+#undef RB_ACCEPT_ARGS
+}

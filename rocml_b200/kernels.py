@@ -221,6 +221,10 @@ def _lib():
         lib.rb_delta_scan_chunks.argtypes = [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i,
                                              _vp, _i, _vp]
         lib.rb_low_rank.argtypes = [_vp, _i, _i, _ll, _i, _i, _i, _vp, _i, _i, _i, _vp, _i, _i, _i, _vp, _i, _vp]
+        lib.rb_attention_tree.argtypes = [_vp, _ll, _i, _vp, _ll, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i,
+                                          _f, _i, _i, _f, _vp, _f, _i, _i, _vp, _vp, _vp, _vp]
+        lib.rb_tree_accept.argtypes = [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _ll, _i, _i, _vp]
+        lib.rb_token_logprobs.argtypes = [_vp, _i, _ll, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _vp]
         lib.rb_gemm_tcgen05_set_wait.argtypes = [_ll, _i]
         lib.rb_gemm_tcgen05_set_wait.restype = None
         _sigs_done = True
@@ -883,6 +887,186 @@ def sample(logits: torch.Tensor, n: int, rows: torch.Tensor, history: Optional[t
         raise KernelError("sample: logits float32 with unit inner stride, out int32, 8 words per row")
     _check(_lib().rb_sample(_ptr(logits), logits.stride(0), n, logits.shape[1], _i32(rows, "rows"),
                             None if history is None else _i32(history, "history"), _ptr(out), _stream()), "sample")
+
+
+# ---- trees of drafted tokens, and scoring ---------------------------------------------------------------------------------
+
+TREE_MAX_NODES = 256       # nodes a tree holds at most (rows of 8 words of bits)
+TREE_MAX_SEQS = 1024       # sequences a call takes
+_TREE_ROWS = 16            # rows of a tile of attention_tree's 32-bit kernel
+
+
+def _here(what: str, *tensors) -> None:
+    """The launch goes to the current device's current stream: every tensor must live there."""
+    device = None
+    for t in tensors:
+        if t is not None:
+            if not t.is_cuda:
+                raise KernelError(f"{what}: arguments must live on a CUDA device; there is no CPU path")
+            if device is None:
+                device = torch._C._cuda_getDevice()
+            if t.get_device() != device:
+                raise KernelError(f"{what}: every tensor must live on the current CUDA device ({device})")
+
+
+def _tree_sizes(what: str, visible, cu_q, n_seqs: int, max_nodes: int) -> int:
+    """The words a row of bits has, after the checks that the tree kernels share."""
+    if visible.dtype != torch.int32 or visible.dim() != 2 or not visible.is_contiguous():
+        raise KernelError(f"{what}: visible must be contiguous int32 [tokens, words]")
+    words = visible.shape[1]
+    if not 1 <= max_nodes <= min(TREE_MAX_NODES, 32 * words) or words > TREE_MAX_NODES // 32:
+        raise KernelError(f"{what}: trees of up to {max_nodes} nodes in {words} words of bits (1 to {TREE_MAX_NODES} nodes, 32 a word)")
+    if not 0 <= n_seqs <= TREE_MAX_SEQS or cu_q.numel() < n_seqs + 1:
+        raise KernelError(f"{what}: {n_seqs} sequences (at most {TREE_MAX_SEQS}, with cu_q of one more)")
+    return words
+
+
+def tree_shares(n_seqs: int, tiles: int, n_pages: int, slots: int) -> int:
+    """How many blocks share the pages that one tile of rows reads (csrc/attention_tree.cu): as many as fill the device once over all
+    tiles, never more than there are pages; with more tiles than blocks run at once, about four waves of blocks."""
+    shares = slots // tiles if tiles <= slots else -(-4 * slots // tiles)
+    return max(1, min(shares, n_seqs * n_pages))
+
+
+@_profiled(lambda a, facts: _attention_cost(a, facts))
+def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                   seq_slot: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, visible: torch.Tensor, n_seqs: int, max_nodes: int,
+                   nq: int, nkv: int, hd: int, scale: float, max_kv_len: Optional[int] = None, positions: Optional[torch.Tensor] = None,
+                   window: int = 0, keep: int = 0, sink=None, softcap: float = 0.0):
+    """Softmax attention of trees of drafted tokens, q rows [T, >= nq * hd] (row stride free) -> out rows, bfloat16 or float32.  Sequence b
+    brings its rows cu_q[b] .. cu_q[b + 1], n of them (at most ``max_nodes``); its context is the kv_len[b] - n positions before them, and row j's key
+    and value already lie at place kv_len[b] - n + j of its pages.  A row sees the whole context and, among the sequence's own rows,
+    those whose bit is set in its row of ``visible`` (int32 [T, words], bit j % 32 of word j / 32): its ancestors and itself, as a rule.
+    ``window`` > 0: of the context only the places above positions[t] - window (``positions`` int32 [T], none below kv_len - n), and those below
+    ``keep``.  ``sink`` and ``softcap`` as in ``attention_generic``.  ``max_kv_len``: the longest sequence, if known (it decides how the work is
+    split, nothing else).  A row that sees nothing is zero.  Rows of slots below 0, of sequences shorter than their tree or longer than their row of the block
+    table stay as they are.  What a row does not see takes no part in its result, whatever it holds; a bfloat16 row that sees a value
+    that is not finite may become NaN as a whole."""
+    words = _tree_sizes("attention_tree", visible, cu_q, n_seqs, max_nodes)
+    if n_seqs == 0:
+        return
+    if q.stride(-1) != 1 or out.stride(-1) != 1 or q.dtype != out.dtype or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise KernelError("attention_tree: strides or types do not fit")
+    if nkv < 1 or nq < 1 or nq % nkv or not 1 <= hd <= 512 or tuple(k_cache.shape[1:]) != (nkv, PAGE, hd) or k_cache.shape != v_cache.shape or \
+            not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise KernelError("attention_tree: cache must be contiguous [pages, nkv, 64, hd], hd at most 512")
+    T = visible.shape[0]
+    if q.dim() != 2 or out.dim() != 2 or q.shape[0] < T or out.shape[0] < T or q.shape[1] < nq * hd or out.shape[1] < nq * hd:
+        raise KernelError("attention_tree: q and out must hold a row of nq * hd for every row of visible")
+    if not scale > 0 or window < 0 or keep < 0 or softcap < 0 or (window > 0 and (positions is None or positions.numel() < T)):
+        raise KernelError("attention_tree: scale is positive, window, keep and softcap are not negative, a window comes with positions")
+    if seq_slot.numel() < n_seqs or kv_len.numel() < n_seqs or block_table.dim() != 2:
+        raise KernelError("attention_tree: seq_slot, kv_len and block_table do not fit")
+    _here("attention_tree", q, out, k_cache, v_cache, block_table, seq_slot, cu_q, kv_len, visible, positions)
+    n_pages = block_table.shape[1]
+    if max_kv_len is not None:
+        n_pages = min(n_pages, max(1, -(-int(max_kv_len) // PAGE)))
+    rows_tile = _TREE_ROWS
+    tiles = nkv * -(-max_nodes * (nq // nkv) // rows_tile)
+    shares = tree_shares(n_seqs, tiles, n_pages, _decode_slots(q.device))
+    acc = ml = None
+    if shares > 1:
+        places = 2 * shares * tiles * rows_tile
+        acc = torch.empty(places * hd, dtype=torch.float32, device=q.device)
+        ml = torch.empty(places * 2, dtype=torch.float32, device=q.device)
+    rc = _lib().rb_attention_tree(
+        _ptr(q), q.stride(0), T, _ptr(out), out.stride(0), dtype_code(q.dtype), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0],
+        _i32(block_table, "block_table"), block_table.shape[1], _i32(seq_slot, "seq_slot"), _i32(cu_q, "cu_q"), _i32(kv_len, "kv_len"),
+        _ptr(visible), words, None if positions is None else _i32(positions, "positions"), n_seqs, max_nodes, nq, nkv, hd, float(scale),
+        int(window), int(keep), *_sink(sink, nq), float(softcap), shares, rows_tile, _ptr(acc), _ptr(ml), _ptr(status_word(q.device)), _stream())
+    _check(rc, "attention_tree")
+
+
+@_profiled(lambda a, facts: _cost.tree_accept(a["token_ids"].numel(), a["n_seqs"]))
+def tree_accept(token_ids: torch.Tensor, parents: torch.Tensor, visible: torch.Tensor, sampled: torch.Tensor, cu_q: torch.Tensor, n_seqs: int,
+                path: torch.Tensor, counts: torch.Tensor, next_token: torch.Tensor, seq_slot: Optional[torch.Tensor] = None,
+                kv_len: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None, k: Optional[torch.Tensor] = None,
+                v: Optional[torch.Tensor] = None):
+    """What of every tree of drafted tokens (int32 ``token_ids``, ``parents`` within the tree, -1 for the first node and any other root, and the
+    rows of ancestor bits ``visible``) the tokens that were sampled at the nodes confirm.  Node 0 always is; a node below it when its parent is
+    and the parent's sampled token is its own (of several such children the first).  path int32 [n_seqs, >= the largest tree] receives the confirmed
+    nodes from node 0 down, -1 behind them, counts [n_seqs] how many they are, next_token [n_seqs] the token sampled at the last one.
+    With ``k`` and ``v`` [layers, pages, nkv, 64, hd] (and seq_slot, kv_len, block_table as for ``attention_tree``) their keys and values are moved
+    to the places kv_len - n + 0, 1, 2, ... in every layer.  Rows of slots below 0 stay as they are.  Parents come before their
+    children."""
+    if path.dim() != 2 or path.shape[0] < n_seqs or not path.is_contiguous():
+        raise KernelError("tree_accept: path must be contiguous int32 [n_seqs, nodes]")
+    words = _tree_sizes("tree_accept", visible, cu_q, n_seqs, min(path.shape[1], 32 * visible.shape[-1]))
+    if n_seqs == 0:
+        return
+    T = visible.shape[0]
+    if token_ids.numel() < T or parents.numel() < T or sampled.numel() < T or counts.numel() < n_seqs or next_token.numel() < n_seqs:
+        raise KernelError("tree_accept: a token, a parent and a sample for every node, counts and next_token for every sequence")
+    if path.shape[1] > TREE_MAX_NODES:
+        raise KernelError(f"tree_accept: path holds at most {TREE_MAX_NODES} nodes a sequence")
+    layers = nkv = row_bytes = esz = 0
+    n_pages = max_pages = 0
+    if (k is None) != (v is None):
+        raise KernelError("tree_accept: keys and values come together")
+    if k is not None:
+        if seq_slot is None or kv_len is None or block_table is None or seq_slot.numel() < n_seqs or kv_len.numel() < n_seqs:
+            raise KernelError("tree_accept: moving keys and values needs seq_slot, kv_len and block_table")
+        if k.dim() != 5 or k.shape[3] != PAGE or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or not v.is_contiguous():
+            raise KernelError("tree_accept: k and v must be contiguous [layers, pages, nkv, 64, hd]")
+        layers, n_pages, nkv = k.shape[0], k.shape[1], k.shape[2]
+        esz = k.element_size()
+        row_bytes, max_pages = k.shape[4] * esz, block_table.shape[1]
+    _here("tree_accept", token_ids, parents, visible, sampled, cu_q, path, counts, next_token, seq_slot, kv_len, block_table, k, v)
+    rc = _lib().rb_tree_accept(
+        _i32(token_ids, "token_ids"), _i32(parents, "parents"), _ptr(visible), words, _i32(sampled, "sampled"), _i32(cu_q, "cu_q"), n_seqs,
+        _i32(path, "path"), path.shape[1], _i32(counts, "counts"), _i32(next_token, "next_token"),
+        None if seq_slot is None else _i32(seq_slot, "seq_slot"), None if kv_len is None else _i32(kv_len, "kv_len"),
+        None if block_table is None else _i32(block_table, "block_table"), max_pages, _ptr(k), _ptr(v), layers, nkv, n_pages, row_bytes, esz,
+        _stream())
+    _check(rc, "tree_accept")
+
+
+LOGPROBS_MAX_TOP = 32
+
+
+def logprob_blocks(rows: int, vocab: int, device=0) -> int:
+    """Blocks a row of token_logprobs: as many as keep the device full once, a power of two up to 16, none with less than 2,048 logits."""
+    slots = 2 * _decode_slots(device) // 3
+    blocks = 1
+    while blocks < 16 and rows * blocks * 2 <= slots and vocab // (blocks * 2) >= 2048:
+        blocks *= 2
+    return blocks
+
+
+@_profiled(lambda a, facts: _cost.token_logprobs(a["logits"].shape[0], a["logits"].shape[1], _esz(a["logits"])))
+def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor], logprobs: Optional[torch.Tensor], entropy: Optional[torch.Tensor] = None,
+                   top_logprobs: Optional[torch.Tensor] = None, top_ids: Optional[torch.Tensor] = None):
+    """Log probabilities (natural) under softmax(logits), logits [n, V] float32 or bfloat16, rows any stride apart.  logprobs float32 [n, m]
+    receives those of the tokens ids int32 [n, m] (-inf for an id outside the vocabulary), entropy float32 [n] the rows' entropy,
+    top_logprobs float32 and top_ids int32 [n, k], k <= 32, the k most likely tokens, most likely first, equal ones by their id.  Any of the three may be
+    None.  A logit of -inf is a token that cannot be; in a row of nothing else every log probability is -inf and the entropy 0.  A row that holds a NaN
+    or +inf gives NaN."""
+    if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < 1:
+        raise KernelError("token_logprobs: logits must be [n, V] with unit inner stride")
+    n, V = logits.shape
+    m = top = 0
+    if (ids is None) != (logprobs is None):
+        raise KernelError("token_logprobs: ids and logprobs come together")
+    if ids is not None:
+        m = ids.shape[1] if ids.dim() == 2 else -1
+        if m < 0 or tuple(ids.shape) != (n, m) or tuple(logprobs.shape) != (n, m) or logprobs.dtype != torch.float32 or not logprobs.is_contiguous():
+            raise KernelError("token_logprobs: ids int32 [n, m], logprobs contiguous float32 [n, m]")
+    if entropy is not None and (entropy.dtype != torch.float32 or entropy.numel() != n or not entropy.is_contiguous()):
+        raise KernelError("token_logprobs: entropy must be contiguous float32 [n]")
+    if (top_logprobs is None) != (top_ids is None):
+        raise KernelError("token_logprobs: top_logprobs and top_ids come together")
+    if top_ids is not None:
+        top = top_ids.shape[1] if top_ids.dim() == 2 else -1
+        if not 0 <= top <= min(LOGPROBS_MAX_TOP, V) or tuple(top_ids.shape) != (n, top) or tuple(top_logprobs.shape) != (n, top) or \
+                top_logprobs.dtype != torch.float32 or not top_logprobs.is_contiguous():
+            raise KernelError(f"token_logprobs: top_ids int32 and top_logprobs float32 [n, k], contiguous, k at most {LOGPROBS_MAX_TOP} and the vocabulary")
+    if n == 0:
+        return
+    _here("token_logprobs", logits, ids, logprobs, entropy, top_logprobs, top_ids)
+    rc = _lib().rb_token_logprobs(
+        _ptr(logits), dtype_code(logits.dtype), logits.stride(0), n, V, None if ids is None else _i32(ids, "ids"), m, _ptr(logprobs), _ptr(entropy),
+        _ptr(top_logprobs), None if top_ids is None else _i32(top_ids, "top_ids"), top, logprob_blocks(n, V, logits.device), _stream())
+    _check(rc, "token_logprobs")
 
 
 # ---- tensor-core matrix product (tcgen05) ----------------------------------------------------------------

@@ -127,3 +127,13 @@ def decoder_flops(tokens: int, hidden: int, q_dim: int, kv_dim: int, inter: int,
     down in every layer, the head on ``logit_rows`` rows) plus the attention's own."""
     per_layer = 2 * tokens * (hidden * (q_dim + 2 * kv_dim) + q_dim * hidden + 3 * hidden * inter)
     return n_layers * per_layer + 2 * logit_rows * hidden * vocab + attention_flops
+
+
+def tree_accept(nodes: int, seqs: int) -> Cost:
+    """Settling drafted trees: a token, a parent, a sample and a word of bits a node; what is moved depends on the samples."""
+    return nodes * 16 + seqs * 8, nodes
+
+
+def token_logprobs(rows: int, vocab: int, esz: int) -> Cost:
+    """Every logit once; a maximum, an exponential, two sums an element."""
+    return rows * vocab * esz, 5 * rows * vocab
