@@ -893,7 +893,7 @@ def sample(logits: torch.Tensor, n: int, rows: torch.Tensor, history: Optional[t
 
 TREE_MAX_NODES = 256       # nodes a tree holds at most (rows of 8 words of bits)
 TREE_MAX_SEQS = 1024       # sequences a call takes
-_TREE_ROWS = 16            # rows of a tile of attention_tree's 32-bit kernel
+_TREE_ROWS = 16            # rows of a tile of attention_tree's plain kernel
 
 
 def _here(what: str, *tensors) -> None:
@@ -961,9 +961,15 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     n_pages = block_table.shape[1]
     if max_kv_len is not None:
         n_pages = min(n_pages, max(1, -(-int(max_kv_len) // PAGE)))
+    group = nq // nkv
+    slots = _decode_slots(q.device)                    # three blocks of the plain kernel a multiprocessor
     rows_tile = _TREE_ROWS
-    tiles = nkv * -(-max_nodes * (nq // nkv) // rows_tile)
-    shares = tree_shares(n_seqs, tiles, n_pages, _decode_slots(q.device))
+    if q.dtype == torch.bfloat16 and hd in (64, 128, 256) and group <= 128 and not \
+            ((q.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15 or (q.stride(0) | out.stride(0)) & 7):
+        rows_tile = 128 // group * group               # the tensor-core kernel: whole nodes in 128 rows
+        slots = slots // 3 * (2 if hd <= 128 else 1)
+    tiles = nkv * -(-max_nodes * group // rows_tile)
+    shares = tree_shares(n_seqs, tiles, n_pages, slots)
     acc = ml = None
     if shares > 1:
         places = 2 * shares * tiles * rows_tile
