@@ -346,13 +346,20 @@ int rb_rglru_step(const float* u, int ld_u, const void* ra, const void* ri, int 
 
 // Attention of trees of drafted tokens over the paged cache (attention_tree.cu): sequence b's nodes are the rows cu_q[b] .. cu_q[b + 1], their keys
 // and values lie at the places kv_len[b] - n + j; row t sees the context (inside `window` of positions[t], and below `keep`) and the nodes whose
-// bits are set in visible[t] (int32 [tokens, words]).  shares: blocks that share a (head, row tile)'s pages; rows_tile: rb_attention_tree_rows;
-// part_o / part_ml: float32 [2 shares, row tiles * nkv, rows_tile, hd] and [.., 2] when shares > 1.
-int rb_attention_tree(const void* q, long long q_stride, int T, void* out, long long o_stride, int dtype, const void* k_cache,
-                      const void* v_cache, int n_pages, const int* block_table, int max_pages, const int* seq_slot, const int* cu_q,
-                      const int* kv_len, const int* visible, int words, const int* positions, int n_seqs, int max_nodes, int nq, int nkv, int hd,
-                      float scale, int window, int keep, float sink, const float* sinks, float softcap, int shares, int rows_tile,
-                      float* part_o, float* part_ml, int* status, void* stream);
+// bits are set in visible[t] (int32 [tokens, words]).  shares: blocks that share a head's pages; rows_tile: 16, or 128 / group * group for
+// the tensor-core kernel.
+typedef struct RbTreeCall {
+    const void *q, *k_cache, *v_cache;
+    void* out;
+    const int *block_table, *seq_slot, *cu_q, *kv_len, *visible, *positions;
+    const float* sinks;
+    float* work;
+    int* status;
+    long long q_stride, o_stride;
+    int tokens, dtype, n_pages, max_pages, words, n_seqs, max_nodes, nq, nkv, hd, window, keep, shares, rows_tile;
+    float scale, sink, softcap;
+} RbTreeCall;
+int rb_attention_tree(const RbTreeCall* call, void* stream);
 
 // Which nodes of every tree the sampled tokens confirm (path [n_seqs, path_ld], counts, next_token) and, when k and v ([layers, n_pages, nkv, 64,
 // row_bytes]) are given, the confirmed nodes' keys and values moved to the places behind the context (tree_accept.cu).

@@ -10,11 +10,11 @@
 // Rows.  The rows of a (sequence, key/value head) are its nodes times the `group` query heads that share the head, node by
 // node: a tile of rows reads every key once for all of them.
 //
-// Shares.  What is read grows with the contexts, and contexts differ.  So for each (key/value head, row tile) the pages of ALL sequences
-// are laid end to end, W of them, and `shares` blocks take W / shares pages each, wherever sequences begin and end: every block
-// streams the same number of pages.  A sequence that lies inside one share is finished there; of one that is cut, each share
-// leaves (maximum, sum, unnormalised result) in the work space and attention_tree_merge_kernel joins them.  A share is cut at most
-// at its two ends, so its work space has two places: 2 c for a sequence that began earlier, 2 c + 1 for one that goes on later.
+// Shares.  What is read grows with the contexts, and contexts differ.  So for each key/value head the pages of ALL sequences (as often as
+// a sequence has tiles of rows) are laid end to end, W of them, and `shares` blocks take W / shares pages each, wherever sequences begin and
+// end: every block streams the same number of pages.  A (sequence, tile of rows) that lies inside one share is finished there; of
+// one that is cut, each share leaves (maximum, sum, unnormalised result) in the work space and attention_tree_merge_kernel joins them.  A
+// share is cut at most at its two ends, so its work space has two places: 2 c for what began earlier, 2 c + 1 for what goes on later.
 //
 // This file: the entry point, the kernel that joins pieces, and attention_tree_simple_kernel, which takes any head size up to 512 and both types
 // with 32-bit multiply-adds.  attention_tree_tc5.cu: bfloat16 heads of 64, 128 and 256 on the tensor cores.
@@ -62,15 +62,18 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
     float* Vs = Ks + 64 * SLD;
     float* Ps = Vs + 64 * SLD;                     // [16][SLD]
     int* pre = (int*)(Ps + SR * SLD);
-    const int tile = blockIdx.y, kvh = tile % a.nkv, mt = tile / a.nkv;
-    prefix_tiles(a, mt, pre);
+    int* tl = pre + a.B + 1;
+    const int kvh = blockIdx.y;
+    prefix_tiles(a, pre, tl);
     Pieces pieces(pre, a.B, a.shares, blockIdx.x);
+    if (a.n_notes) note_nothing(a, pieces, pre, tl, kvh, blockIdx.x, threadIdx.x, 128);
     const int rg = threadIdx.x >> 4, kg = threadIdx.x & 15;
     const float sl2 = a.scale * LOG2E;
     const rb::SoftCap capped = rb::soft_cap(a.scale, a.softcap);
-    int b, p0, p1;
-    while (pieces.next(pre, b, p0, p1)) {
-        const Seq s = seq_of(a, b, mt);
+    int b, mt, p0, p1;
+    while (pieces.next(pre, tl, b, mt, p0, p1)) {
+        const Seq s = seq_of(a, b);
+        if (a.n_notes && threadIdx.x == 0) note_piece(a, pieces, s, kvh, blockIdx.x, b, mt, p0, p1);
         const int row0 = mt * a.rows_tile, rows = min(SR, s.n * a.group - row0);
         const int* table = a.block_table + (size_t)s.slot * a.max_pages;
         __syncthreads();
@@ -189,7 +192,7 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
                     for (int e = 0; e < 4; ++e)
                         if (c * 64 + 4 * kg + e < a.hd) dst[c * 64 + 4 * kg + e] = rb::from_f32<T>(o[c][r][e] * inv);
             } else {
-                const size_t place = ((size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * gridDim.y + tile) * a.rows_tile + 2 * rg + r;
+                const size_t place = ((size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * a.nkv + kvh) * a.rows_tile + 2 * rg + r;
                 if (kg == 0) { a.part_ml[place * 2] = m[r]; a.part_ml[place * 2 + 1] = l[r]; }
 #pragma unroll
                 for (int c = 0; c < BLOCKS; ++c)
@@ -201,77 +204,80 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
     }
 }
 
-// ---- joining what several shares have of a sequence --------------------------------------------------------------------
-// A warp a row.  Grid (row tiles times quarters of a tile's rows, nkv, sequences).
-template <typename T>
+// ---- joining what several shares have of a (sequence, tile of rows) -----------------------------------------------------
+// Block (x, head, entry) joins rows 8 x .. 8 x + 7 of what the entry's note names, a warp two rows: the shares' maxima and sums 32 at
+// a time, a lane each, then their results, the whole head side by side and eight shares in flight.
+constexpr int MERGE_ROWS = 8;
+template <typename T, int VEC>              // VEC: dimensions a lane, 32 VEC >= hd
 __global__ void __launch_bounds__(128)
-attention_tree_merge_kernel(T* __restrict__ out, long long o_stride, int n_tiles_y, const TreeArgs a) {
+attention_tree_merge_kernel(T* __restrict__ out, long long o_stride, const TreeArgs a) {
     rb::pdl_trigger();
     rb::pdl_wait();
-    __shared__ int sums[2][4];
-    const int b = blockIdx.z, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per_tile = (a.rows_tile + 3) / 4;
-    const int mt = blockIdx.x / per_tile, r = blockIdx.x % per_tile * 4 + warp, row = mt * a.rows_tile + r;
-    // the tiles before this sequence, and all
-    int before = 0, all = 0;
-    for (int i = threadIdx.x; i < a.B; i += 128) {
-        const int t = seq_of(a, i, mt).tiles;
-        all += t;
-        if (i < b) before += t;
-    }
+    const int kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int4 note = *note_of(a, kvh, blockIdx.z);
+    const int c0 = note.w >> 16, c1 = note.w & 0xffff;
+    if (c0 == c1) return;
+    for (int r = blockIdx.x * MERGE_ROWS + warp; r < min(note.z, (int)(blockIdx.x + 1) * MERGE_ROWS); r += 4) {
+        const int row = note.y + r;
+        const int node = row / a.group, head = kvh * a.group + row % a.group;
+        auto place = [&](int c) { return ((size_t)(2 * c + (c == c0 ? 1 : 0)) * a.nkv + kvh) * a.rows_tile + r; };
+        const float sink = (a.sinks ? a.sinks[head] : a.sink) * LOG2E;
+        float top = rb::has_sink(sink) ? sink : NEG_BIG, total = rb::has_sink(sink) ? 1.f : 0.f;
+        float acc[VEC];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-        all += __shfl_xor_sync(0xffffffffu, all, o);
-    }
-    if (lane == 0) { sums[0][warp] = before; sums[1][warp] = all; }
-    __syncthreads();
-    before = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
-    const long long W = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
-    const Seq s = seq_of(a, b, mt);
-    if (s.tiles == 0 || r >= a.rows_tile || row >= s.n * a.group) return;
-    // share of page f: the last c with c W / shares <= f
-    const long long shares = min((long long)a.shares, W);
-    const int c0 = (int)((((long long)before + 1) * shares - 1) / W);
-    const int c1 = (int)((((long long)before + s.tiles) * shares - 1) / W);
-    if (c0 == c1) return;                                     // finished where it lies
-    const int tile = mt * a.nkv + kvh;
-    const int node = row / a.group, head = kvh * a.group + row % a.group;
-    auto place = [&](int c) { return ((size_t)(2 * c + (c == c0 ? 1 : 0)) * n_tiles_y + tile) * a.rows_tile + r; };
-    float top = NEG_BIG;
-    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, a.part_ml[place(c) * 2]);
-    top = rb::warp_max(top);
-    const float sink = (a.sinks ? a.sinks[head] : a.sink) * LOG2E;
-    if (rb::has_sink(sink)) top = fmaxf(top, sink);
-    float total = 0.f;
-    for (int c = c0 + lane; c <= c1; c += 32) total += a.part_ml[place(c) * 2 + 1] * exp2f(a.part_ml[place(c) * 2] - top);
-    total = rb::warp_sum(total);
-    if (rb::has_sink(sink)) total += exp2f(sink - top);
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    T* dst = out + (size_t)(s.q0 + node) * o_stride + (size_t)head * a.hd;
-    for (int d0 = 0; d0 < a.hd; d0 += 128) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int c = c0; c <= c1; ++c) {
-            const size_t pl = place(c);
-            const float f = exp2f(a.part_ml[pl * 2] - top);
+        for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+        const int d0 = lane * VEC;
+        for (int g = c0; g <= c1; g += 32) {
+            const int n = min(32, c1 - g + 1);
+            float m = NEG_BIG, l = 0.f;
+            if (lane < n) {
+                const float2 x = *reinterpret_cast<const float2*>(a.part_ml + place(g + lane) * 2);
+                m = x.x;
+                l = x.y;
+            }
+            const float top_new = fmaxf(top, rb::warp_max(m)), old = exp2f(top - top_new), f = exp2f(m - top_new);
+            total = total * old + rb::warp_sum(lane < n ? l * f : 0.f);
+            top = top_new;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int d = d0 + lane + 32 * e;
-                if (d < a.hd) acc[e] = fmaf(f, a.part_o[pl * a.hd + d], acc[e]);
+            for (int e = 0; e < VEC; ++e) acc[e] *= old;
+            for (int i0 = 0; i0 < n; i0 += 8) {
+                float x[8][VEC];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float* src = a.part_o + place(g + min(i0 + i, n - 1)) * a.hd + d0;
+                    if constexpr (VEC % 4 == 0) {
+#pragma unroll
+                        for (int e = 0; e < VEC; e += 4)
+                            if (i0 + i < n && d0 + e < a.hd) rb::load4(src + e, x[i] + e);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e)
+                            if (i0 + i < n && d0 + e < a.hd) x[i][e] = src[e];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float w = __shfl_sync(0xffffffffu, f, min(i0 + i, 31));
+                    if (i0 + i < n) {
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e)
+                            if (d0 + e < a.hd) acc[e] = fmaf(w, x[i][e], acc[e]);
+                    }
+                }
             }
         }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        T* dst = out + (size_t)(note.x + node) * o_stride + (size_t)head * a.hd + d0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int d = d0 + lane + 32 * e;
-            if (d < a.hd) dst[d] = rb::from_f32<T>(acc[e] * inv);
-        }
+        for (int e = 0; e < VEC; ++e)
+            if (d0 + e < a.hd) dst[e] = rb::from_f32<T>(acc[e] * inv);
     }
 }
 
 template <typename T, int BLOCKS>
-int launch_simple(const void* q, long long q_stride, void* out, long long o_stride, const void* k, const void* v, int tiles, const TreeArgs& a,
+int launch_simple(const void* q, long long q_stride, void* out, long long o_stride, const void* k, const void* v, const TreeArgs& a,
                   cudaStream_t stream) {
-    const size_t smem = (SR * 64 * BLOCKS + 2 * 64 * SLD + SR * SLD) * sizeof(float) + (a.B + 1) * sizeof(int);
+    const size_t smem = (SR * 64 * BLOCKS + 2 * 64 * SLD + SR * SLD) * sizeof(float) + (2 * a.B + 1) * sizeof(int);
     auto kernel = attention_tree_simple_kernel<T, BLOCKS>;
     static rb::PerDevice<int> allowed;
     int device;
@@ -283,56 +289,74 @@ int launch_simple(const void* q, long long q_stride, void* out, long long o_stri
         return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
     });
     if (rc) return rc;
-    RB_LAUNCH((kernel), dim3(a.shares, tiles), dim3(128), smem, stream, (const T*)q, q_stride, (T*)out, o_stride, (const T*)k, (const T*)v, a);
+    RB_LAUNCH((kernel), dim3(a.shares, a.nkv), dim3(128), smem, stream, (const T*)q, q_stride, (T*)out, o_stride, (const T*)k, (const T*)v, a);
     return RB_OK;
 }
 
 template <typename T>
-int launch_any(const void* q, long long q_stride, void* out, long long o_stride, const void* k, const void* v, int tiles, const TreeArgs& a,
+int launch_any(const void* q, long long q_stride, void* out, long long o_stride, const void* k, const void* v, const TreeArgs& a,
                cudaStream_t stream) {
-    if (a.hd <= 64) return launch_simple<T, 1>(q, q_stride, out, o_stride, k, v, tiles, a, stream);
-    if (a.hd <= 128) return launch_simple<T, 2>(q, q_stride, out, o_stride, k, v, tiles, a, stream);
-    if (a.hd <= 256) return launch_simple<T, 4>(q, q_stride, out, o_stride, k, v, tiles, a, stream);
-    return launch_simple<T, 8>(q, q_stride, out, o_stride, k, v, tiles, a, stream);
+    if (a.hd <= 64) return launch_simple<T, 1>(q, q_stride, out, o_stride, k, v, a, stream);
+    if (a.hd <= 128) return launch_simple<T, 2>(q, q_stride, out, o_stride, k, v, a, stream);
+    if (a.hd <= 256) return launch_simple<T, 4>(q, q_stride, out, o_stride, k, v, a, stream);
+    return launch_simple<T, 8>(q, q_stride, out, o_stride, k, v, a, stream);
 }
 
 template <typename T>
-int launch_merge(void* out, long long o_stride, int tiles, const TreeArgs& a, cudaStream_t stream) {
-    RB_LAUNCH((attention_tree_merge_kernel<T>), dim3(tiles / a.nkv * ((a.rows_tile + 3) / 4), a.nkv, a.B), dim3(128), 0, stream, (T*)out, o_stride, tiles, a);
+int launch_merge(void* out, long long o_stride, const TreeArgs& a, cudaStream_t stream) {
+    const dim3 grid((a.rows_tile + MERGE_ROWS - 1) / MERGE_ROWS, a.nkv, a.n_notes);
+    // four dimensions a lane are read together where heads are a whole number of them
+    if (a.hd <= 32) RB_LAUNCH((attention_tree_merge_kernel<T, 1>), grid, dim3(128), 0, stream, (T*)out, o_stride, a);
+    else if (a.hd <= 128 && a.hd % 4 == 0) RB_LAUNCH((attention_tree_merge_kernel<T, 4>), grid, dim3(128), 0, stream, (T*)out, o_stride, a);
+    else if (a.hd <= 256 && a.hd % 4 == 0) RB_LAUNCH((attention_tree_merge_kernel<T, 8>), grid, dim3(128), 0, stream, (T*)out, o_stride, a);
+    else if (a.hd % 4 == 0) RB_LAUNCH((attention_tree_merge_kernel<T, 16>), grid, dim3(128), 0, stream, (T*)out, o_stride, a);
+    else RB_LAUNCH((attention_tree_merge_kernel<T, 17>), grid, dim3(128), 0, stream, (T*)out, o_stride, a);
     return RB_OK;
 }
 }  // namespace
 
-// rows_tile: 16, the plain kernel; 128 / group * group, the tensor-core kernel (attention_tree_tc5.cu), which takes aligned rows only.
-extern "C" int rb_attention_tree(const void* q, long long q_stride, int T, void* out, long long o_stride, int dtype, const void* k_cache,
-                                 const void* v_cache, int n_pages, const int* block_table, int max_pages, const int* seq_slot, const int* cu_q,
-                                 const int* kv_len, const int* visible, int words, const int* positions, int n_seqs, int max_nodes, int nq,
-                                 int nkv, int hd, float scale, int window, int keep, float sink, const float* sinks, float softcap,
-                                 int shares, int rows_tile, float* part_o, float* part_ml, int* status, void* stream) {
-    if (n_seqs <= 0 || max_nodes <= 0) return RB_OK;
-    if (n_seqs > MAX_SEQS || nkv <= 0 || nq <= 0 || nq % nkv || hd <= 0 || hd > 512 || words <= 0 || shares <= 0 || window < 0 ||
-        keep < 0 || !(scale > 0.f) || max_pages <= 0 || (window > 0 && !positions) || (shares > 1 && (!part_o || !part_ml)))
+// rows_tile: 16, the plain kernel; 128 / group * group, the tensor-core kernel (attention_tree_tc5.cu), which takes aligned rows only.  work (shares > 1,
+// 16-byte aligned): 2 shares * nkv * rows_tile * (hd + 2) floats, then nkv * min(shares - 1, n_seqs * tiles of rows of max_nodes nodes) entries
+// of four ints.
+extern "C" int rb_attention_tree(const RbTreeCall* call, void* stream) {
+    const RbTreeCall& x = *call;
+    if (x.n_seqs <= 0 || x.max_nodes <= 0) return RB_OK;
+    if (x.n_seqs > MAX_SEQS || x.nkv <= 0 || x.nq <= 0 || x.nq % x.nkv || x.hd <= 0 || x.hd > 512 || x.words <= 0 || x.max_nodes > 32 * x.words ||
+        x.shares <= 0 || x.shares > 32767 || x.window < 0 || x.keep < 0 || !(x.scale > 0.f) || x.max_pages <= 0 || (x.window > 0 && !x.positions) ||
+        (x.shares > 1 && !x.work) || x.nkv > 65535 || x.rows_tile <= 0)
         return RB_ERR_BAD_SIZE;
-    if (dtype != RB_F32 && dtype != RB_BF16) return RB_ERR_BAD_DTYPE;
-    if (window == 0) keep = 0;
-    const int group = nq / nkv;
-    const bool tc5 = rows_tile != SR;
-    if (tc5 && (dtype != RB_BF16 || (hd != 64 && hd != 128 && hd != 256) || group > 128 || rows_tile != 128 / group * group)) return RB_ERR_BAD_SIZE;
-    TreeArgs a{block_table, max_pages, seq_slot, cu_q, kv_len, visible, words, positions, n_seqs, nq, nkv, group, hd,
-               scale, window, keep, sink, sinks, softcap, shares, rows_tile, part_o, part_ml};
-    const long long m_tiles = ((long long)max_nodes * group + rows_tile - 1) / rows_tile;
-    if (m_tiles * nkv > 65535) return RB_ERR_BAD_SIZE;
-    const int tiles = (int)m_tiles * nkv;
+    if (x.dtype != RB_F32 && x.dtype != RB_BF16) return RB_ERR_BAD_DTYPE;
+    if ((uintptr_t)x.work & 15) return RB_ERR_BAD_ALIGN;
+    const int group = x.nq / x.nkv;
+    const bool tc5 = x.rows_tile != SR;
+    if (tc5 && (x.dtype != RB_BF16 || (x.hd != 64 && x.hd != 128 && x.hd != 256) || group > 128 || x.rows_tile != 128 / group * group)) return RB_ERR_BAD_SIZE;
+    TreeArgs a{};
+    a.block_table = x.block_table; a.max_pages = x.max_pages; a.seq_slot = x.seq_slot; a.cu_q = x.cu_q; a.kv_len = x.kv_len;
+    a.visible = x.visible; a.words = x.words; a.positions = x.positions;
+    a.B = x.n_seqs; a.nq = x.nq; a.nkv = x.nkv; a.group = group; a.hd = x.hd;
+    a.scale = x.scale; a.window = x.window; a.keep = x.window > 0 ? x.keep : 0; a.sink = x.sink; a.sinks = x.sinks; a.softcap = x.softcap;
+    a.shares = x.shares; a.rows_tile = x.rows_tile; a.max_nodes = x.max_nodes;
+    const long long units = ((long long)x.max_nodes * group + x.rows_tile - 1) / x.rows_tile;
+    if (units > 0x7fffffff / MAX_SEQS) return RB_ERR_BAD_SIZE;
+    a.max_units = (int)units;
+    if (x.shares > 1) {
+        const size_t places = 2ull * x.shares * x.nkv * x.rows_tile;
+        a.part_o = x.work;
+        a.part_ml = x.work + places * x.hd;
+        a.notes = reinterpret_cast<int4*>(a.part_ml + places * 2);
+        a.notes_by_unit = x.n_seqs * units < x.shares - 1;
+        a.n_notes = a.notes_by_unit ? (int)(x.n_seqs * units) : x.shares - 1;
+    }
     cudaStream_t st = (cudaStream_t)stream;
     int rc;
     if (tc5) {
-        rc = launch_tc5(q, q_stride, T, out, o_stride, k_cache, v_cache, n_pages, tiles, a, status, st);
+        rc = launch_tc5(x.q, x.q_stride, x.tokens, x.out, x.o_stride, x.k_cache, x.v_cache, x.n_pages, a, x.status, st);
     } else {
-        const int align = dtype == RB_F32 ? 15 : 7;
-        if (hd % 4 == 0 && (((uintptr_t)k_cache & align) || ((uintptr_t)v_cache & align))) return RB_ERR_BAD_ALIGN;
-        rc = dtype == RB_F32 ? launch_any<float>(q, q_stride, out, o_stride, k_cache, v_cache, tiles, a, st)
-                             : launch_any<__nv_bfloat16>(q, q_stride, out, o_stride, k_cache, v_cache, tiles, a, st);
+        const int align = x.dtype == RB_F32 ? 15 : 7;
+        if (x.hd % 4 == 0 && (((uintptr_t)x.k_cache & align) || ((uintptr_t)x.v_cache & align))) return RB_ERR_BAD_ALIGN;
+        rc = x.dtype == RB_F32 ? launch_any<float>(x.q, x.q_stride, x.out, x.o_stride, x.k_cache, x.v_cache, a, st)
+                               : launch_any<__nv_bfloat16>(x.q, x.q_stride, x.out, x.o_stride, x.k_cache, x.v_cache, a, st);
     }
-    if (rc != RB_OK || shares == 1) return rc;
-    return dtype == RB_F32 ? launch_merge<float>(out, o_stride, tiles, a, st) : launch_merge<__nv_bfloat16>(out, o_stride, tiles, a, st);
+    if (rc != RB_OK || x.shares == 1) return rc;
+    return x.dtype == RB_F32 ? launch_merge<float>(x.out, x.o_stride, a, st) : launch_merge<__nv_bfloat16>(x.out, x.o_stride, a, st);
 }

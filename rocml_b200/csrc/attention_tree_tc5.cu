@@ -31,7 +31,7 @@ struct Sizes {
     static constexpr int STAGES = HD == 64 ? 4 : 2;
     static constexpr int BLOCKS_PER_SM = HD <= 128 ? 2 : 1;
     static constexpr int TILE_BYTES = Q_HALF * HALVES + 2 * STAGES * KV_TILE;
-    static constexpr int EXTRA = 1024 + 512 + (MAX_SEQS + 1) * 4;      // alignment, barriers, prefix sums
+    static constexpr int EXTRA = 1024 + 512 + (2 * MAX_SEQS + 1) * 4;  // alignment, barriers, the sequences' tiles and their sums
     static constexpr int SMEM_BYTES = TILE_BYTES + EXTRA;
     static_assert(BLOCKS_PER_SM * (SMEM_BYTES + 1024) <= 228 * 1024, "the blocks must fit a multiprocessor");
     static constexpr int TMEM_COLS = HD <= 128 ? 256 : 512;      // S0 [0, 64), S1 [64, 128), O [128, 128 + HD)
@@ -94,7 +94,8 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     auto* bar = (Barriers<STAGES>*)(Vs + STAGES * KV_TILE);
     static_assert(sizeof(Barriers<STAGES>) <= 512, "barriers");
     int* pre = (int*)(Vs + STAGES * KV_TILE + 512);
-    const int tile = blockIdx.y, kvh = tile % a.nkv, mt = tile / a.nkv, row0 = mt * a.rows_tile;
+    int* tl = pre + a.B + 1;
+    const int kvh = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -119,19 +120,19 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tmem_relinquish();
     }
     tc_fence_before();
-    prefix_tiles(a, mt, pre);              // (ends with a block-wide barrier)
+    prefix_tiles(a, pre, tl);              // (ends with a block-wide barrier)
     tc_fence_after();
     const uint32_t tmem_base = bar->tmem_slot;
     Pieces pieces(pre, a.B, a.shares, blockIdx.x);
-    int b, p0, p1;
+    int b, mt, p0, p1;
 
     if (warp == 0) {
         if (lane == 0) { tma_prefetch_desc(&map_q); tma_prefetch_desc(&map_k); tma_prefetch_desc(&map_v); }
         const int q_bytes = a.rows_tile * 128 * HALVES;
         bool ok = true;
         int it = 0, piece = 0;             // tiles and pieces so far
-        while (ok && pieces.next(pre, b, p0, p1)) {
-            const Seq s = seq_of(a, b, mt);
+        while (ok && pieces.next(pre, tl, b, mt, p0, p1)) {
+            const Seq s = seq_of(a, b);
             const int* table = a.block_table + (size_t)s.slot * a.max_pages;
             int page = 0;
             for (int j = p0; j < p1 && ok; ++j, ++it) {
@@ -151,7 +152,7 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                                 mbar_arrive_expect_tx(&bar->q_full, q_bytes);
 #pragma unroll
                                 for (int h = 0; h < HALVES; ++h)
-                                    tma_load_3d(Qs + h * Q_HALF, &map_q, h * 64, kvh * a.group, s.q0 + row0 / a.group, &bar->q_full);
+                                    tma_load_3d(Qs + h * Q_HALF, &map_q, h * 64, kvh * a.group, s.q0 + mt * (a.rows_tile / a.group), &bar->q_full);
                             }
                         }
                         ok = ok && mbar_wait(&bar->v_empty[st], free_parity);
@@ -201,7 +202,7 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                 mma_commit(&bar->s_full[t & 1]);
                 return true;
             };
-            while (ok && pieces.next(pre, b, p0, p1)) {
+            while (ok && pieces.next(pre, tl, b, mt, p0, p1)) {
                 const int n = p1 - p0;
                 ok = mbar_wait(&bar->q_full, piece & 1);
                 if (ok) { tc_fence_after(); ok = issue_s(it, it - 1, n == 1); }
@@ -236,18 +237,17 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         const rb::SoftCap capped = rb::soft_cap(a.scale, a.softcap);
         bool alive = true;
         int it = 0, piece = 0, checks = 0;      // tiles, pieces and masked tiles so far
-        while (alive && pieces.next(pre, b, p0, p1)) {
-            const Seq s = seq_of(a, b, mt);
-            const int rows = min(a.rows_tile, s.n * a.group - row0);
+        if (a.n_notes) note_nothing(a, pieces, pre, tl, kvh, blockIdx.x, tid, 128);
+        while (alive && pieces.next(pre, tl, b, mt, p0, p1)) {
+            const Seq s = seq_of(a, b);
+            const int row0 = mt * a.rows_tile, rows = min(a.rows_tile, s.n * a.group - row0);
+            if (a.n_notes && tid == 0) note_piece(a, pieces, s, kvh, blockIdx.x, b, mt, p0, p1);
             const bool row_here = r < rows, warp_here = quarter * 32 < rows;
             const int node = (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
             float m_used = NEG_BIG, l_sum = 0.f;
             for (int j = p0; j < p1; ++j, ++it) {
                 const int buf = it & 1, st = it % STAGES;
                 const int key0 = tile_of(s, j) * BK;
-                alive = __all_sync(0xffffffffu, wait_or_abort(&bar->s_full[buf], (it >> 1) & 1, &bar->abort_flag));
-                if (!alive) break;
-                tc_fence_after();
                 // a tile inside the context that every node sees whole needs no mask (no position is behind the sequence's last)
                 const bool whole_tile = key0 + BK <= s.ctx && (a.window == 0 || key0 >= s.len - a.window || key0 + BK <= a.keep);
                 unsigned long long seen = ~0ull;
@@ -286,6 +286,9 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                     spoiled = (seen & (((unsigned long long)bad[1] << 32) | bad[0])) != 0;
                     ++checks;
                 }
+                alive = __all_sync(0xffffffffu, wait_or_abort(&bar->s_full[buf], (it >> 1) & 1, &bar->abort_flag));
+                if (!alive) break;
+                tc_fence_after();
                 if (warp_here) {
                     float sv[BK];
                     tmem_ld64(lane_base + buf * BK, sv);
@@ -363,7 +366,7 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                     if (rb::has_sink(sink)) l_sum += exp2f(fminf(sink - m_used, 126.f));
                 }
                 const float f = !whole ? 1.f : l_sum == 0.f ? 0.f : 1.f / l_sum;
-                const size_t place = ((size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * gridDim.y + tile) * a.rows_tile + r;
+                const size_t place = ((size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * a.nkv + kvh) * a.rows_tile + r;
                 __nv_bfloat16* orow = out + (size_t)(s.q0 + node) * o_stride + (size_t)head * HD;
                 float* prow = a.part_o + place * HD;
                 if (!whole && row_here) { a.part_ml[place * 2] = m_used; a.part_ml[place * 2 + 1] = l_sum; }
@@ -411,7 +414,7 @@ int encode(CUtensorMap* map, const void* ptr, int dims, const cuuint64_t* size, 
 }
 
 template <int HD, bool CAP>
-int launch(const void* q, long long q_stride, int T, void* out, long long o_stride, const void* k, const void* v, int n_pages, int tiles,
+int launch(const void* q, long long q_stride, int T, void* out, long long o_stride, const void* k, const void* v, int n_pages,
            const TreeArgs& a, int* status, cudaStream_t stream) {
     CUtensorMap mq, mk, mv;
     const cuuint64_t q_size[3] = {(cuuint64_t)HD, (cuuint64_t)a.nq, (cuuint64_t)T}, q_strides[2] = {(cuuint64_t)HD * 2, (cuuint64_t)q_stride * 2};
@@ -430,17 +433,17 @@ int launch(const void* q, long long q_stride, int T, void* out, long long o_stri
     const int* known;
     rc = allowed.get(device, &known, [&](int&) { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sizes<HD>::SMEM_BYTES); });
     if (rc) return rc;
-    RB_LAUNCH((kernel), dim3(a.shares, tiles), dim3(192), Sizes<HD>::SMEM_BYTES, stream, mq, mk, mv, (__nv_bfloat16*)out, o_stride, a, status);
+    RB_LAUNCH((kernel), dim3(a.shares, a.nkv), dim3(192), Sizes<HD>::SMEM_BYTES, stream, mq, mk, mv, (__nv_bfloat16*)out, o_stride, a, status);
     return RB_OK;
 }
 }  // namespace
 
 namespace rb_tree {
-int launch_tc5(const void* q, long long q_stride, int T, void* out, long long o_stride, const void* k, const void* v, int n_pages, int tiles,
+int launch_tc5(const void* q, long long q_stride, int T, void* out, long long o_stride, const void* k, const void* v, int n_pages,
                const TreeArgs& a, int* status, cudaStream_t stream) {
     if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) || q_stride % 8 || o_stride % 8) return RB_ERR_BAD_ALIGN;
     if (T <= 0 || n_pages <= 0 || !status || (long long)n_pages * a.nkv * PAGE > 0x7fffffffll) return RB_ERR_BAD_SIZE;
-#define RB_TREE_ARGS q, q_stride, T, out, o_stride, k, v, n_pages, tiles, a, status, stream
+#define RB_TREE_ARGS q, q_stride, T, out, o_stride, k, v, n_pages, a, status, stream
     if (a.softcap > 0.f)
         return a.hd == 64 ? launch<64, true>(RB_TREE_ARGS) : a.hd == 128 ? launch<128, true>(RB_TREE_ARGS) : launch<256, true>(RB_TREE_ARGS);
     return a.hd == 64 ? launch<64, false>(RB_TREE_ARGS) : a.hd == 128 ? launch<128, false>(RB_TREE_ARGS) : launch<256, false>(RB_TREE_ARGS);

@@ -17,12 +17,14 @@ struct TreeArgs {
     int B, nq, nkv, group, hd;
     float scale; int window, keep; float sink; const float* sinks; float softcap;
     int shares, rows_tile;           // rows_tile: rows of a tile that are used, a whole number of nodes for the tensor-core kernel
-    float* part_o; float* part_ml;   // [2 shares][gridDim.y tiles][rows_tile][hd], [..][2]
+    int max_nodes, max_units;        // nodes and tiles of rows of the largest tree
+    int4* notes; int n_notes, notes_by_unit;      // see note_of
+    float* part_o; float* part_ml;   // [2 shares][nkv][rows_tile][hd], [..][2]
 };
 
-struct Seq { int slot, q0, n, ctx, len, first, kept, tiles; };   // tiles of 64 keys: [0, kept) and [first, ..]
+struct Seq { int slot, q0, n, ctx, len, first, kept, tiles, units; };   // tiles of 64 keys: [0, kept) and [first, ..]; units: tiles of rows
 
-__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int b, int mt) {
+__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int b) {
     Seq s;
     s.slot = a.seq_slot[b];
     s.q0 = a.cu_q[b];
@@ -30,63 +32,113 @@ __device__ __forceinline__ Seq seq_of(const TreeArgs& a, int b, int mt) {
     s.len = a.kv_len[b];
     s.ctx = s.len - s.n;
     // (a sequence shorter than its nodes, or longer than its row of the table, is no sequence: nothing is read or written for it)
-    const bool live = s.slot >= 0 && s.n > 0 && s.ctx >= 0 && s.len <= a.max_pages * PAGE && mt * a.rows_tile < s.n * a.group;
+    const bool live = s.slot >= 0 && s.n > 0 && s.n <= a.max_nodes && s.ctx >= 0 && s.len <= a.max_pages * PAGE;
     const int lo = a.window > 0 ? max(0, s.ctx - a.window + 1) : 0;       // (positions are >= ctx)
     s.first = min(lo, s.ctx) / PAGE;
     s.kept = a.keep > 0 ? min((a.keep + PAGE - 1) / PAGE, s.first) : 0;
     s.tiles = live ? s.kept + (s.len - 1) / PAGE - s.first + 1 : 0;
+    s.units = live ? (s.n * a.group + a.rows_tile - 1) / a.rows_tile : 0;
     return s;
 }
 __device__ __forceinline__ int tile_of(const Seq& s, int j) { return j < s.kept ? j : s.first + (j - s.kept); }
 
-// pre[b] = tiles of the sequences before b, pre[B] = all of them.  Every thread of the block calls this.
-__device__ __forceinline__ void prefix_tiles(const TreeArgs& a, int mt, int* pre) {
-    for (int b = threadIdx.x; b < a.B; b += blockDim.x) pre[b + 1] = seq_of(a, b, mt).tiles;
+// pre[b] = (tile of keys, tile of rows) pairs of the sequences before b, pre[B] = all of them; tl[b] = tiles of keys of sequence b.  Every thread
+// of the block calls this.
+__device__ __forceinline__ void prefix_tiles(const TreeArgs& a, int* pre, int* tl) {
+    for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
+        const Seq s = seq_of(a, b);
+        tl[b] = s.tiles;
+        pre[b + 1] = s.tiles * s.units;
+    }
     if (threadIdx.x == 0) pre[0] = 0;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        int carry = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 32) {
-            const int b = b0 + threadIdx.x;
-            int v = b < a.B ? pre[b + 1] : 0;
+    if (a.B > 1) {
+        if (threadIdx.x < 32) {
+            int carry = 0;
+            for (int b0 = 0; b0 < a.B; b0 += 32) {
+                const int b = b0 + threadIdx.x;
+                int v = b < a.B ? pre[b + 1] : 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, v, o);
-                if ((int)threadIdx.x >= o) v += u;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(0xffffffffu, v, o);
+                    if ((int)threadIdx.x >= o) v += u;
+                }
+                if (b < a.B) pre[b + 1] = carry + v;
+                carry += __shfl_sync(0xffffffffu, v, 31);
             }
-            if (b < a.B) pre[b + 1] = carry + v;
-            carry += __shfl_sync(0xffffffffu, v, 31);
         }
+        __syncthreads();
     }
-    __syncthreads();
+}
+// The sequence that holds pair f (f < pre[B]).
+__device__ __forceinline__ int sequence_of(const int* pre, int B, int f) {
+    int lo = 0, hi = B - 1;
+    while (lo < hi) {                      // the last b with pre[b] <= f
+        const int mid = (lo + hi + 1) >> 1;
+        if (pre[mid] <= f) lo = mid; else hi = mid - 1;
+    }
+    return lo;
 }
 
-// Walks the pieces of sequences that one share holds.
+// Walks the pieces that one share holds: of a sequence's tiles of rows one after the other, each over all its tiles of keys.
 struct Pieces {
-    int f, end, b;
-    __device__ Pieces(const int* pre, int B, int shares, int c) {
-        const long long W = pre[B];
-        if (shares > W) shares = max(1, (int)W);           // (no share between two others is empty: the joining kernel counts on it)
-        f = c < shares ? (int)(c * W / shares) : 0;
-        end = c < shares ? (int)((c + 1) * W / shares) : 0;
-        int lo = 0, hi = B - 1;
-        while (lo < hi) {                      // the last b with pre[b] <= f (the one that holds page f)
-            const int mid = (lo + hi + 1) >> 1;
-            if (pre[mid] <= f) lo = mid; else hi = mid - 1;
-        }
-        b = lo;
+    int f, end, b, W, shares;
+    __device__ Pieces(const int* pre, int B, int n_shares, int c) {
+        W = pre[B];
+        shares = max(1, min(n_shares, W));           // (no share between two others is empty: joining counts on it)
+        f = c < shares ? (int)((long long)c * W / shares) : 0;
+        end = c < shares ? (int)((c + 1ll) * W / shares) : 0;
+        b = sequence_of(pre, B, f);
     }
-    // the next piece: tiles [p0, p1) of sequence `seq`; false: none is left
-    __device__ bool next(const int* pre, int& seq, int& p0, int& p1) {
+    // the next piece: tiles of keys [p0, p1) for tile of rows mt of sequence `seq`; false: none is left
+    __device__ bool next(const int* pre, const int* tl, int& seq, int& mt, int& p0, int& p1) {
         if (f >= end) return false;
         while (pre[b + 1] <= f) ++b;
         seq = b;
-        p0 = f - pre[b];
-        p1 = min(pre[b + 1], end) - pre[b];
+        const int t = tl[b], off = f - pre[b];
+        mt = off / t;
+        p0 = off - mt * t;
+        p1 = min(t, p0 + end - f);
         f += p1 - p0;
         return true;
     }
+    // the share that holds pair g: the last c with c W / shares <= g
+    __device__ int share_of(int g) const { return (int)(((g + 1ll) * shares - 1) / W); }
 };
+
+// What the joining kernel is told, one entry a (sequence, tile of rows) where those are fewer than the shares, else one a share (for what begins in it
+// and goes on in the next): {first token, first row, rows, first share << 16 | last share}; equal shares: nothing to join.
+__device__ __forceinline__ int4* note_of(const TreeArgs& a, int kvh, int entry) { return a.notes + (size_t)kvh * a.n_notes + entry; }
+// One thread of a block calls this for every piece.
+__device__ __forceinline__ void note_piece(const TreeArgs& a, const Pieces& p, const Seq& s, int kvh, int c, int b, int mt, int p0, int p1) {
+    if (p0 != 0) return;
+    const int last = p1 == s.tiles ? c : p.share_of(p.f - p1 + s.tiles - 1);
+    const int row0 = mt * a.rows_tile;
+    const int4 note = make_int4(s.q0, row0, min(a.rows_tile, s.n * a.group - row0), (c << 16) | last);
+    if (a.notes_by_unit) *note_of(a, kvh, b * a.max_units + mt) = note;
+    else if (last != c) *note_of(a, kvh, c) = note;
+}
+// Every thread of a block calls this once: entries that no piece will fill.
+__device__ __forceinline__ void note_nothing(const TreeArgs& a, const Pieces& p, const int* pre, const int* tl, int kvh, int c, int tid, int threads) {
+    const int4 none = make_int4(0, 0, 0, 0);
+    if (a.notes_by_unit) {
+        if (c == 0)
+            for (int u = tid; u < a.n_notes; u += threads) {
+                const int b = u / a.max_units;
+                if (tl[b] == 0 || (u % a.max_units) * tl[b] >= pre[b + 1] - pre[b]) *note_of(a, kvh, u) = none;
+            }
+        return;
+    }
+    // by shares: this one has an entry unless its end cuts what began in it
+    if (tid == 0 && c < a.n_notes) {
+        bool cuts = false;
+        if (c + 1 < p.shares && p.f < p.end) {
+            const int b = sequence_of(pre, a.B, p.end), begin = p.end - (p.end - pre[b]) % tl[b];
+            cuts = begin != p.end && begin >= p.f;
+        }
+        if (!cuts) *note_of(a, kvh, c) = none;
+    }
+}
 
 // Bits [a, b) of 64 (a and b may lie outside).
 __device__ __forceinline__ unsigned long long range_bits(int a, int b) {
@@ -118,6 +170,6 @@ __device__ __forceinline__ unsigned long long seen_bits(const TreeArgs& a, int t
 }
 
 // attention_tree_tc5.cu: bfloat16, head sizes 64, 128 and 256; rows_tile = 128 / group * group.
-int launch_tc5(const void* q, long long q_stride, int T, void* out, long long o_stride, const void* k, const void* v, int n_pages, int tiles,
+int launch_tc5(const void* q, long long q_stride, int T, void* out, long long o_stride, const void* k, const void* v, int n_pages,
                const TreeArgs& a, int* status, cudaStream_t stream);
 }  // namespace rb_tree

@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import inspect
+import struct
 from typing import Optional
 
 import torch
@@ -221,8 +222,7 @@ def _lib():
         lib.rb_delta_scan_chunks.argtypes = [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i,
                                              _vp, _i, _vp]
         lib.rb_low_rank.argtypes = [_vp, _i, _i, _ll, _i, _i, _i, _vp, _i, _i, _i, _vp, _i, _i, _i, _vp, _i, _vp]
-        lib.rb_attention_tree.argtypes = [_vp, _ll, _i, _vp, _ll, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i,
-                                          _f, _i, _i, _f, _vp, _f, _i, _i, _vp, _vp, _vp, _vp]
+        lib.rb_attention_tree.argtypes = [_c.c_char_p, _vp]
         lib.rb_tree_accept.argtypes = [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _ll, _i, _i, _vp]
         lib.rb_token_logprobs.argtypes = [_vp, _i, _ll, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _vp]
         lib.rb_gemm_tcgen05_set_wait.argtypes = [_ll, _i]
@@ -898,34 +898,42 @@ _TREE_ROWS = 16            # rows of a tile of attention_tree's plain kernel
 
 def _here(what: str, *tensors) -> None:
     """The launch goes to the current device's current stream: every tensor must live there."""
-    device = None
+    device = tensors[0].get_device()
     for t in tensors:
-        if t is not None:
-            if not t.is_cuda:
-                raise KernelError(f"{what}: arguments must live on a CUDA device; there is no CPU path")
-            if device is None:
-                device = torch._C._cuda_getDevice()
-            if t.get_device() != device:
-                raise KernelError(f"{what}: every tensor must live on the current CUDA device ({device})")
+        if t is not None and t.get_device() != device:
+            raise KernelError(f"{what}: every tensor must live on one device")
+    if device < 0:
+        raise KernelError(f"{what}: arguments must live on a CUDA device; there is no CPU path")
+    if device != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: its tensors live on device {device}, which is not the current one")
 
 
-def _tree_sizes(what: str, visible, cu_q, n_seqs: int, max_nodes: int) -> int:
-    """The words a row of bits has, after the checks that the tree kernels share."""
-    if visible.dtype != torch.int32 or visible.dim() != 2 or not visible.is_contiguous():
-        raise KernelError(f"{what}: visible must be contiguous int32 [tokens, words]")
-    words = visible.shape[1]
-    if not 1 <= max_nodes <= min(TREE_MAX_NODES, 32 * words) or words > TREE_MAX_NODES // 32:
+def _ints(what: str, *tensors) -> None:
+    for t in tensors:
+        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()):
+            raise KernelError(f"{what}: ids, lengths, tables and bits must be contiguous int32 tensors")
+
+
+def _tree_sizes(what: str, visible, cu_q, n_seqs: int, max_nodes: int):
+    """(tokens, words of bits a token), after the checks that the tree kernels share."""
+    if visible.dim() != 2:
+        raise KernelError(f"{what}: visible must be [tokens, words]")
+    tokens, words = visible.shape
+    if words > TREE_MAX_NODES // 32 or not 1 <= max_nodes <= 32 * words:
         raise KernelError(f"{what}: trees of up to {max_nodes} nodes in {words} words of bits (1 to {TREE_MAX_NODES} nodes, 32 a word)")
-    if not 0 <= n_seqs <= TREE_MAX_SEQS or cu_q.numel() < n_seqs + 1:
+    if not 0 <= n_seqs <= TREE_MAX_SEQS or cu_q.numel() <= n_seqs:
         raise KernelError(f"{what}: {n_seqs} sequences (at most {TREE_MAX_SEQS}, with cu_q of one more)")
-    return words
+    return tokens, words
 
 
-def tree_shares(n_seqs: int, tiles: int, n_pages: int, slots: int) -> int:
-    """How many blocks share the pages that one tile of rows reads (csrc/attention_tree.cu): as many as fill the device once over all
-    tiles, never more than there are pages; with more tiles than blocks run at once, about four waves of blocks."""
-    shares = slots // tiles if tiles <= slots else -(-4 * slots // tiles)
-    return max(1, min(shares, n_seqs * n_pages))
+# RbTreeCall of csrc/api.h (one packed argument: converting thirty costs microseconds)
+_TREE_CALL = struct.Struct("@13P2q14i3f")
+
+
+def tree_shares(pairs: int, nkv: int, slots: int) -> int:
+    """How many blocks a key/value head's work is shared among (csrc/attention_tree.cu): as many as fill the device once over all heads, never
+    more than there are (page, tile of rows) pairs; with more heads than blocks run at once, about four waves of blocks."""
+    return max(1, min(slots // nkv if nkv <= slots else -(-4 * slots // nkv), pairs))
 
 
 @_profiled(lambda a, facts: _attention_cost(a, facts))
@@ -942,45 +950,50 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     split, nothing else).  A row that sees nothing is zero.  Rows of slots below 0, of sequences shorter than their tree or longer than their row of the block
     table stay as they are.  What a row does not see takes no part in its result, whatever it holds; a bfloat16 row that sees a value
     that is not finite may become NaN as a whole."""
-    words = _tree_sizes("attention_tree", visible, cu_q, n_seqs, max_nodes)
-    if n_seqs == 0:
-        return
-    if q.stride(-1) != 1 or out.stride(-1) != 1 or q.dtype != out.dtype or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
-        raise KernelError("attention_tree: strides or types do not fit")
-    if nkv < 1 or nq < 1 or nq % nkv or not 1 <= hd <= 512 or tuple(k_cache.shape[1:]) != (nkv, PAGE, hd) or k_cache.shape != v_cache.shape or \
+    tokens, words = _tree_sizes("attention_tree", visible, cu_q, n_seqs, max_nodes)
+    dtype = q.dtype
+    if dtype is not out.dtype or dtype is not k_cache.dtype or dtype is not v_cache.dtype:
+        raise KernelError("attention_tree: q, out and the cache must have one type")
+    if nkv < 1 or nq < 1 or nq % nkv or not 1 <= hd <= 512 or k_cache.shape[1:] != (nkv, PAGE, hd) or k_cache.shape != v_cache.shape or \
             not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise KernelError("attention_tree: cache must be contiguous [pages, nkv, 64, hd], hd at most 512")
-    T = visible.shape[0]
-    if q.dim() != 2 or out.dim() != 2 or q.shape[0] < T or out.shape[0] < T or q.shape[1] < nq * hd or out.shape[1] < nq * hd:
-        raise KernelError("attention_tree: q and out must hold a row of nq * hd for every row of visible")
-    if not scale > 0 or window < 0 or keep < 0 or softcap < 0 or (window > 0 and (positions is None or positions.numel() < T)):
+    if q.dim() != 2 or out.dim() != 2:
+        raise KernelError("attention_tree: q and out must be rows")
+    (q_rows, q_width), (o_rows, o_width) = q.shape, out.shape
+    (q_stride, q_inner), (o_stride, o_inner) = q.stride(), out.stride()
+    if q_rows < tokens or o_rows < tokens or q_width < nq * hd or o_width < nq * hd or q_inner != 1 or o_inner != 1:
+        raise KernelError("attention_tree: q and out must hold a row of nq * hd, unit stride, for every row of visible")
+    if not scale > 0 or window < 0 or keep < 0 or softcap < 0 or (window > 0 and (positions is None or positions.numel() < tokens)):
         raise KernelError("attention_tree: scale is positive, window, keep and softcap are not negative, a window comes with positions")
     if seq_slot.numel() < n_seqs or kv_len.numel() < n_seqs or block_table.dim() != 2:
         raise KernelError("attention_tree: seq_slot, kv_len and block_table do not fit")
+    _ints("attention_tree", block_table, seq_slot, cu_q, kv_len, visible, positions)
     _here("attention_tree", q, out, k_cache, v_cache, block_table, seq_slot, cu_q, kv_len, visible, positions)
-    n_pages = block_table.shape[1]
-    if max_kv_len is not None:
-        n_pages = min(n_pages, max(1, -(-int(max_kv_len) // PAGE)))
+    if n_seqs == 0:
+        return
+    one_sink, sinks = _sink(sink, nq)
+    max_pages = block_table.shape[1]
+    longest = max_pages if max_kv_len is None else max(1, min(max_pages, (int(max_kv_len) + PAGE - 1) // PAGE))
+    device = q.device
     group = nq // nkv
-    slots = _decode_slots(q.device)                    # three blocks of the plain kernel a multiprocessor
+    slots = _decode_slots(device)                      # three blocks of the plain kernel a multiprocessor
     rows_tile = _TREE_ROWS
-    if q.dtype == torch.bfloat16 and hd in (64, 128, 256) and group <= 128 and not \
-            ((q.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15 or (q.stride(0) | out.stride(0)) & 7):
+    pointers = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+    if dtype is torch.bfloat16 and hd in (64, 128, 256) and group <= 128 and not \
+            ((pointers[0] | pointers[1] | pointers[2] | pointers[3]) & 15 or (q_stride | o_stride) & 7):
         rows_tile = 128 // group * group               # the tensor-core kernel: whole nodes in 128 rows
         slots = slots // 3 * (2 if hd <= 128 else 1)
-    tiles = nkv * -(-max_nodes * group // rows_tile)
-    shares = tree_shares(n_seqs, tiles, n_pages, slots)
-    acc = ml = None
+    units = n_seqs * -(-max_nodes * group // rows_tile)
+    shares = tree_shares(longest * units, nkv, slots)
+    work = None
     if shares > 1:
-        places = 2 * shares * tiles * rows_tile
-        acc = torch.empty(places * hd, dtype=torch.float32, device=q.device)
-        ml = torch.empty(places * 2, dtype=torch.float32, device=q.device)
-    rc = _lib().rb_attention_tree(
-        _ptr(q), q.stride(0), T, _ptr(out), out.stride(0), dtype_code(q.dtype), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0],
-        _i32(block_table, "block_table"), block_table.shape[1], _i32(seq_slot, "seq_slot"), _i32(cu_q, "cu_q"), _i32(kv_len, "kv_len"),
-        _ptr(visible), words, None if positions is None else _i32(positions, "positions"), n_seqs, max_nodes, nq, nkv, hd, float(scale),
-        int(window), int(keep), *_sink(sink, nq), float(softcap), shares, rows_tile, _ptr(acc), _ptr(ml), _ptr(status_word(q.device)), _stream())
-    _check(rc, "attention_tree")
+        work = torch.empty(2 * shares * nkv * rows_tile * (hd + 2) + 4 * nkv * min(shares - 1, units), dtype=torch.float32, device=device)
+    call = _TREE_CALL.pack(
+        *pointers, block_table.data_ptr(), seq_slot.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
+        0 if positions is None else positions.data_ptr(), sinks or 0, 0 if work is None else work.data_ptr(), status_word(device).data_ptr(),
+        q_stride, o_stride, tokens, dtype_code(dtype), k_cache.shape[0], max_pages, words, n_seqs, max_nodes, nq, nkv, hd, int(window), int(keep),
+        shares, rows_tile, scale, one_sink, softcap)
+    _check(_lib().rb_attention_tree(call, _stream()), "attention_tree")
 
 
 @_profiled(lambda a, facts: _cost.tree_accept(a["token_ids"].numel(), a["n_seqs"]))
@@ -995,12 +1008,9 @@ def tree_accept(token_ids: torch.Tensor, parents: torch.Tensor, visible: torch.T
     With ``k`` and ``v`` [layers, pages, nkv, 64, hd] (and seq_slot, kv_len, block_table as for ``attention_tree``) their keys and values are moved
     to the places kv_len - n + 0, 1, 2, ... in every layer.  Rows of slots below 0 stay as they are.  Parents come before their
     children."""
-    if path.dim() != 2 or path.shape[0] < n_seqs or not path.is_contiguous():
-        raise KernelError("tree_accept: path must be contiguous int32 [n_seqs, nodes]")
-    words = _tree_sizes("tree_accept", visible, cu_q, n_seqs, min(path.shape[1], 32 * visible.shape[-1]))
-    if n_seqs == 0:
-        return
-    T = visible.shape[0]
+    if path.dim() != 2 or path.shape[0] < n_seqs or visible.dim() != 2:
+        raise KernelError("tree_accept: path must be [n_seqs, nodes], visible [tokens, words]")
+    T, words = _tree_sizes("tree_accept", visible, cu_q, n_seqs, min(path.shape[1], 32 * visible.shape[-1]))
     if token_ids.numel() < T or parents.numel() < T or sampled.numel() < T or counts.numel() < n_seqs or next_token.numel() < n_seqs:
         raise KernelError("tree_accept: a token, a parent and a sample for every node, counts and next_token for every sequence")
     if path.shape[1] > TREE_MAX_NODES:
@@ -1017,13 +1027,15 @@ def tree_accept(token_ids: torch.Tensor, parents: torch.Tensor, visible: torch.T
         layers, n_pages, nkv = k.shape[0], k.shape[1], k.shape[2]
         esz = k.element_size()
         row_bytes, max_pages = k.shape[4] * esz, block_table.shape[1]
+    _ints("tree_accept", token_ids, parents, visible, sampled, cu_q, path, counts, next_token, seq_slot, kv_len, block_table)
     _here("tree_accept", token_ids, parents, visible, sampled, cu_q, path, counts, next_token, seq_slot, kv_len, block_table, k, v)
+    if n_seqs == 0:
+        return
+    pointer = lambda t: None if t is None else t.data_ptr()
     rc = _lib().rb_tree_accept(
-        _i32(token_ids, "token_ids"), _i32(parents, "parents"), _ptr(visible), words, _i32(sampled, "sampled"), _i32(cu_q, "cu_q"), n_seqs,
-        _i32(path, "path"), path.shape[1], _i32(counts, "counts"), _i32(next_token, "next_token"),
-        None if seq_slot is None else _i32(seq_slot, "seq_slot"), None if kv_len is None else _i32(kv_len, "kv_len"),
-        None if block_table is None else _i32(block_table, "block_table"), max_pages, _ptr(k), _ptr(v), layers, nkv, n_pages, row_bytes, esz,
-        _stream())
+        token_ids.data_ptr(), parents.data_ptr(), visible.data_ptr(), words, sampled.data_ptr(), cu_q.data_ptr(), n_seqs, path.data_ptr(), path.shape[1],
+        counts.data_ptr(), next_token.data_ptr(), pointer(seq_slot), pointer(kv_len), pointer(block_table), max_pages, pointer(k), pointer(v),
+        layers, nkv, n_pages, row_bytes, esz, _stream())
     _check(rc, "tree_accept")
 
 
@@ -1055,7 +1067,7 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor], logprobs: 
         raise KernelError("token_logprobs: ids and logprobs come together")
     if ids is not None:
         m = ids.shape[1] if ids.dim() == 2 else -1
-        if m < 0 or tuple(ids.shape) != (n, m) or tuple(logprobs.shape) != (n, m) or logprobs.dtype != torch.float32 or not logprobs.is_contiguous():
+        if m < 0 or ids.shape != (n, m) or logprobs.shape != (n, m) or logprobs.dtype != torch.float32 or not logprobs.is_contiguous():
             raise KernelError("token_logprobs: ids int32 [n, m], logprobs contiguous float32 [n, m]")
     if entropy is not None and (entropy.dtype != torch.float32 or entropy.numel() != n or not entropy.is_contiguous()):
         raise KernelError("token_logprobs: entropy must be contiguous float32 [n]")
@@ -1063,15 +1075,17 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor], logprobs: 
         raise KernelError("token_logprobs: top_logprobs and top_ids come together")
     if top_ids is not None:
         top = top_ids.shape[1] if top_ids.dim() == 2 else -1
-        if not 0 <= top <= min(LOGPROBS_MAX_TOP, V) or tuple(top_ids.shape) != (n, top) or tuple(top_logprobs.shape) != (n, top) or \
+        if not 0 <= top <= min(LOGPROBS_MAX_TOP, V) or top_ids.shape != (n, top) or top_logprobs.shape != (n, top) or \
                 top_logprobs.dtype != torch.float32 or not top_logprobs.is_contiguous():
             raise KernelError(f"token_logprobs: top_ids int32 and top_logprobs float32 [n, k], contiguous, k at most {LOGPROBS_MAX_TOP} and the vocabulary")
     if n == 0:
         return
+    _ints("token_logprobs", ids, top_ids)
     _here("token_logprobs", logits, ids, logprobs, entropy, top_logprobs, top_ids)
+    pointer = lambda t: None if t is None else t.data_ptr()
     rc = _lib().rb_token_logprobs(
-        _ptr(logits), dtype_code(logits.dtype), logits.stride(0), n, V, None if ids is None else _i32(ids, "ids"), m, _ptr(logprobs), _ptr(entropy),
-        _ptr(top_logprobs), None if top_ids is None else _i32(top_ids, "top_ids"), top, logprob_blocks(n, V, logits.device), _stream())
+        logits.data_ptr(), dtype_code(logits.dtype), logits.stride(0), n, V, pointer(ids), m, pointer(logprobs), pointer(entropy),
+        pointer(top_logprobs), pointer(top_ids), top, logprob_blocks(n, V, logits.device), _stream())
     _check(rc, "token_logprobs")
 
 

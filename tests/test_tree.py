@@ -9,53 +9,78 @@ from rocml_b200 import kernels
 from rocml_b200.errors import KernelError
 
 
-def pieces_of(tiles, shares):
-    """What csrc/attention_tree.cu's blocks do with sequences of so many tiles: {share: [(sequence, first, end)]}."""
+def pieces_of(sizes, shares):
+    """What csrc/attention_tree.cu's blocks do with sequences of so many (tiles of keys, tiles of rows): {share: [(sequence, tile of rows, first, end)]}."""
     pre = [0]
-    for t in tiles:
-        pre.append(pre[-1] + t)
+    for t, u in sizes:
+        pre.append(pre[-1] + t * u)
     out, shares = {}, max(1, min(shares, pre[-1]))
     for c in range(shares):
         f, end = c * pre[-1] // shares, (c + 1) * pre[-1] // shares
-        lo, hi = 0, len(tiles) - 1
-        while lo < hi:
-            mid = (lo + hi + 1) >> 1
-            lo, hi = (mid, hi) if pre[mid] <= f else (lo, mid - 1)
-        b, got = lo, []
+        b, got = sequence_of(pre, f), []
         while f < end:
             while pre[b + 1] <= f:
                 b += 1
-            p0, p1 = f - pre[b], min(pre[b + 1], end) - pre[b]
-            got.append((b, p0, p1))
+            mt, p0 = divmod(f - pre[b], sizes[b][0])
+            p1 = min(sizes[b][0], p0 + end - f)
+            got.append((b, mt, p0, p1))
             f += p1 - p0
         out[c] = got
     return pre, out, shares
 
 
+def sequence_of(pre, f):
+    lo, hi = 0, len(pre) - 2
+    while lo < hi:
+        mid = (lo + hi + 1) >> 1
+        lo, hi = (mid, hi) if pre[mid] <= f else (lo, mid - 1)
+    return lo
+
+
 @pytest.mark.parametrize("seed", range(60))
 def test_shares_cover_every_tile_once_and_pieces_have_places_of_their_own(seed):
     rng = random.Random(seed)
-    tiles = [rng.choice([0, 1, 2, 3, rng.randrange(1, 200)]) for _ in range(rng.randrange(1, 40))]
+    sizes = [(t, rng.choice([1, 1, 2, 5]) if t else 0) for t in [rng.choice([0, 1, 2, 3, rng.randrange(1, 200)]) for _ in range(rng.randrange(1, 40))]]
     shares = rng.choice([1, 2, 3, 17, 18, 37, 296])
-    pre, pieces, shares = pieces_of(tiles, shares)
-    seen = {b: [] for b in range(len(tiles))}
-    places = {}
+    pre, pieces, shares = pieces_of(sizes, shares)
+    W = pre[-1]
+    seen, places = {}, {}
     for c, got in pieces.items():
-        for b, p0, p1 in got:
-            assert 0 <= p0 < p1 <= tiles[b]
-            seen[b] += range(p0, p1)
-            if not (p0 == 0 and p1 == tiles[b]):
+        for b, mt, p0, p1 in got:
+            assert 0 <= p0 < p1 <= sizes[b][0] and 0 <= mt < sizes[b][1]
+            seen.setdefault((b, mt), []).extend(range(p0, p1))
+            if not (p0 == 0 and p1 == sizes[b][0]):
                 place = 2 * c + (1 if p0 == 0 else 0)
                 assert place < 2 * shares and place not in places        # nobody else's, inside the work space
-                places[place] = (b, c)
-    for b, t in enumerate(tiles):
-        assert sorted(seen[b]) == list(range(t))
-        if t == 0:
-            continue
-        # what the joining kernel works out from the prefix sums alone
-        c0, c1 = ((pre[b] + 1) * shares - 1) // pre[-1], ((pre[b] + t) * shares - 1) // pre[-1]
-        mine = sorted(p for p, (s, _) in places.items() if s == b)
-        assert mine == ([] if c0 == c1 else sorted([2 * c0 + 1] + [2 * c for c in range(c0 + 1, c1 + 1)]))
+                places[place] = (b, mt)
+    for b, (t, u) in enumerate(sizes):
+        for mt in range(u):
+            assert sorted(seen.pop((b, mt))) == list(range(t))
+    assert not seen
+    # the notes that the joining kernel reads: one a (sequence, tile of rows), or one a share
+    share_of = lambda g: ((g + 1) * shares - 1) // W
+    by_unit, by_share, joined = {}, {}, {}
+    for c, got in pieces.items():
+        f, end = c * W // shares, (c + 1) * W // shares
+        for b, mt, p0, p1 in got:
+            if p0 == 0:
+                last = c if p1 == sizes[b][0] else share_of(pre[b] + mt * sizes[b][0] + sizes[b][0] - 1)
+                assert (b, mt) not in by_unit
+                by_unit[b, mt] = (c, last)
+                if last != c:
+                    assert c not in by_share
+                    by_share[c] = (b, mt, last)
+        cuts = False
+        if c + 1 < shares and f < end:
+            b = sequence_of(pre, end)
+            begin = end - (end - pre[b]) % sizes[b][0]
+            cuts = begin != end and begin >= f
+        assert cuts == (c in by_share)
+    for (b, mt), (c0, c1) in by_unit.items():
+        for c in range(c0, c1 + 1) if c0 != c1 else ():
+            joined[2 * c + (1 if c == c0 else 0)] = (b, mt)
+    assert joined == places and sorted(by_unit) == [(b, mt) for b, (_, u) in enumerate(sizes) for mt in range(u)]
+    assert {(b, mt): (c, last) for c, (b, mt, last) in by_share.items()} == {k: v for k, v in by_unit.items() if v[0] != v[1]}
 
 
 @pytest.mark.parametrize("off", [-63, -64, -33, -32, -31, -1, 0, 1, 31, 32, 63, 64, 200, 255])
@@ -96,10 +121,10 @@ def test_confirmed_nodes_by_bits_are_the_walk(seed):
 
 
 def test_shares_fill_the_device_and_never_outnumber_the_pages():
-    assert kernels.tree_shares(1, 8, 200, 444) == 55
-    assert kernels.tree_shares(1, 8, 3, 444) == 3
-    assert kernels.tree_shares(32, 1000, 10, 444) == 2
-    assert kernels.tree_shares(1, 5000, 1, 444) == 1
+    assert kernels.tree_shares(200, 8, 296) == 37
+    assert kernels.tree_shares(3, 8, 296) == 3
+    assert kernels.tree_shares(320, 1000, 296) == 2
+    assert kernels.tree_shares(1, 5000, 296) == 1
 
 
 def _attention(**change):
@@ -121,7 +146,7 @@ def _attention(**change):
     ({"n_seqs": 3}, "3 sequences"),
     ({"nq": 7}, "cache must be"),
     ({"hd": 32}, "cache must be"),
-    ({"q": torch.zeros((5, 512), dtype=torch.bfloat16)}, "types"),
+    ({"q": torch.zeros((5, 512), dtype=torch.bfloat16)}, "one type"),
     ({"scale": 0.0}, "scale is positive"),
     ({"window": 5}, "positions"),
     ({"window": -5}, "not negative"),
