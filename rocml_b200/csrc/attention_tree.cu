@@ -274,6 +274,65 @@ attention_tree_merge_kernel(T* __restrict__ out, long long o_stride, const TreeA
     }
 }
 
+// The tensor-core kernel's results: [hd][rows] a place, a lane a row (that kernel's threads hold a row each, so what a warp writes or reads at once
+// is one line of 32 rows).  Block (x, head, entry): 32 rows by 16 dimensions; warp w takes every eighth share from the w-th on, relative to its own
+// maximum, so that all shares are asked for at once, and the warps meet in shared memory.  (One warp over all shares in turn waited for memory
+// once a share: 14 us with twelve of them.)
+constexpr int JOIN_DIMS = 16, JOIN_WARPS = 8;
+__global__ void __launch_bounds__(32 * JOIN_WARPS)
+attention_tree_merge_rows_kernel(__nv_bfloat16* __restrict__ out, long long o_stride, const TreeArgs a) {
+    rb::pdl_trigger();
+    rb::pdl_wait();
+    __shared__ float part[JOIN_WARPS][JOIN_DIMS][33], tops[JOIN_WARPS][32], sums[JOIN_WARPS][32];
+    const int kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row_blocks = (a.rows_tile + 31) / 32, r0 = blockIdx.x % row_blocks * 32, d0 = blockIdx.x / row_blocks * JOIN_DIMS;
+    const int4 note = *note_of(a, kvh, blockIdx.z);
+    const int c0 = note.w >> 16, c1 = note.w & 0xffff;
+    if (c0 == c1 || r0 >= note.z) return;
+    const int r = min(r0 + lane, note.z - 1);
+    auto place = [&](int c) { return (size_t)(2 * c + (c == c0 ? 1 : 0)) * a.nkv + kvh; };
+    float top = NEG_BIG, total = 0.f, acc[JOIN_DIMS];
+#pragma unroll
+    for (int d = 0; d < JOIN_DIMS; ++d) acc[d] = 0.f;
+#pragma unroll 2
+    for (int c = c0 + warp; c <= c1; c += JOIN_WARPS) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (place(c) * a.rows_tile + r) * 2);
+        const float* src = a.part_o + (place(c) * a.hd + d0) * a.rows_tile + r;
+        float x[JOIN_DIMS];
+#pragma unroll
+        for (int d = 0; d < JOIN_DIMS; ++d) x[d] = src[(size_t)d * a.rows_tile];
+        const float top_new = fmaxf(top, ml.x), old = exp2f(top - top_new), w = exp2f(ml.x - top_new);
+        top = top_new;
+        total = fmaf(total, old, ml.y * w);
+#pragma unroll
+        for (int d = 0; d < JOIN_DIMS; ++d) acc[d] = fmaf(acc[d], old, x[d] * w);
+    }
+    tops[warp][lane] = top;
+    sums[warp][lane] = total;
+#pragma unroll
+    for (int d = 0; d < JOIN_DIMS; ++d) part[warp][d][lane] = acc[d];
+    __syncthreads();
+    // a thread two neighbouring dimensions of a row
+    const int rr = threadIdx.x / (JOIN_DIMS / 2), d = threadIdx.x % (JOIN_DIMS / 2) * 2, row = note.y + r0 + rr;
+    static_assert(32 * JOIN_WARPS == 32 * JOIN_DIMS / 2, "a thread two outputs");
+    if (r0 + rr >= note.z) return;
+    const int node = row / a.group, head = kvh * a.group + row % a.group;
+    const float sink = (a.sinks ? a.sinks[head] : a.sink) * LOG2E;
+    float m = rb::has_sink(sink) ? sink : NEG_BIG;
+#pragma unroll
+    for (int w = 0; w < JOIN_WARPS; ++w) m = fmaxf(m, tops[w][rr]);
+    float l = rb::has_sink(sink) ? exp2f(sink - m) : 0.f, y0 = 0.f, y1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < JOIN_WARPS; ++w) {
+        const float f = exp2f(tops[w][rr] - m);
+        l = fmaf(sums[w][rr], f, l);
+        y0 = fmaf(part[w][d][rr], f, y0);
+        y1 = fmaf(part[w][d + 1][rr], f, y1);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<__nv_bfloat162*>(out + (size_t)(note.x + node) * o_stride + (size_t)head * a.hd + d0 + d) = __floats2bfloat162_rn(y0 * inv, y1 * inv);
+}
+
 template <typename T, int BLOCKS>
 int launch_simple(const void* q, long long q_stride, void* out, long long o_stride, const void* k, const void* v, const TreeArgs& a,
                   cudaStream_t stream) {
@@ -358,5 +417,9 @@ extern "C" int rb_attention_tree(const RbTreeCall* call, void* stream) {
                                : launch_any<__nv_bfloat16>(x.q, x.q_stride, x.out, x.o_stride, x.k_cache, x.v_cache, a, st);
     }
     if (rc != RB_OK || x.shares == 1) return rc;
+    if (tc5) {
+        RB_LAUNCH((attention_tree_merge_rows_kernel), dim3((x.rows_tile + 31) / 32 * (x.hd / JOIN_DIMS), x.nkv, a.n_notes), dim3(32 * JOIN_WARPS), 0, st, (__nv_bfloat16*)x.out, x.o_stride, a);
+        return RB_OK;
+    }
     return x.dtype == RB_F32 ? launch_merge<float>(x.out, x.o_stride, a, st) : launch_merge<__nv_bfloat16>(x.out, x.o_stride, a, st);
 }

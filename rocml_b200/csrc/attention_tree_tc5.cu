@@ -366,10 +366,11 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                     if (rb::has_sink(sink)) l_sum += exp2f(fminf(sink - m_used, 126.f));
                 }
                 const float f = !whole ? 1.f : l_sum == 0.f ? 0.f : 1.f / l_sum;
-                const size_t place = ((size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * a.nkv + kvh) * a.rows_tile + r;
+                // (a place's result is [HD][rows]: a warp writes 32 rows of a dimension as one line)
+                const size_t place = (size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * a.nkv + kvh;
                 __nv_bfloat16* orow = out + (size_t)(s.q0 + node) * o_stride + (size_t)head * HD;
-                float* prow = a.part_o + place * HD;
-                if (!whole && row_here) { a.part_ml[place * 2] = m_used; a.part_ml[place * 2 + 1] = l_sum; }
+                float* prow = a.part_o + place * HD * a.rows_tile + r;
+                if (!whole && row_here) *reinterpret_cast<float2*>(a.part_ml + (place * a.rows_tile + r) * 2) = make_float2(m_used, l_sum);
 #pragma unroll 1
                 for (int c = 0; c < HD / 16; ++c) {
                     float ov[16];
@@ -386,7 +387,7 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                         reinterpret_cast<uint4*>(orow + c * 16)[1] = make_uint4(w[4], w[5], w[6], w[7]);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) rb::store4(prow + c * 16 + 4 * i, ov + 4 * i);
+                        for (int i = 0; i < 16; ++i) prow[(size_t)(c * 16 + i) * a.rows_tile] = ov[i];
                     }
                 }
             }
