@@ -64,8 +64,8 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
     int* pre = (int*)(Ps + SR * SLD);
     int* tl = pre + a.B + 1;
     const int kvh = blockIdx.y;
-    prefix_tiles(a, pre, tl);
-    Pieces pieces(pre, a.B, a.shares, blockIdx.x);
+    const int extra = prefix_tiles(a, pre, tl);
+    Pieces pieces(pre, a.B, a.shares, blockIdx.x, extra);
     if (a.n_notes) note_nothing(a, pieces, pre, tl, kvh, blockIdx.x, threadIdx.x, 128);
     const int rg = threadIdx.x >> 4, kg = threadIdx.x & 15;
     const float sl2 = a.scale * LOG2E;
@@ -86,6 +86,10 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
             }
             Qs[i] = x;
         }
+        RowBits bits[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+            if (2 * rg + r < rows) bits[r].load(a, s.q0 + (row0 + 2 * rg + r) / a.group);
         float m[2] = {NEG_BIG, NEG_BIG}, l[2] = {0.f, 0.f}, o[BLOCKS][2][4];
 #pragma unroll
         for (int c = 0; c < BLOCKS; ++c)
@@ -120,8 +124,7 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
             }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int row = row0 + 2 * rg + r;
-                const unsigned long long seen = 2 * rg + r < rows ? seen_bits(a, s.q0 + row / a.group, s.ctx, s.n, key0) : 0ull;
+                const unsigned long long seen = 2 * rg + r < rows ? bits[r].seen(a, s.ctx, s.n, key0) : 0ull;
                 float mx = NEG_BIG;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -274,10 +277,10 @@ attention_tree_merge_kernel(T* __restrict__ out, long long o_stride, const TreeA
     }
 }
 
-// The tensor-core kernel's results: [hd][rows] a place, a lane a row (that kernel's threads hold a row each, so what a warp writes or reads at once
-// is one line of 32 rows).  Block (x, head, entry): 32 rows by 16 dimensions; warp w takes every eighth share from the w-th on, relative to its own
-// maximum, so that all shares are asked for at once, and the warps meet in shared memory.  (One warp over all shares in turn waited for memory
-// once a share: 14 us with twelve of them.)
+// The tensor-core kernel's results: [hd / 4][rows][4] a place, a lane a row (that kernel's threads hold a row each, so what a warp writes or reads at
+// once is 32 rows' 16 bytes side by side).  A block takes 32 rows.  Its eight warps are `ways` over the shares (the power of two that the number of shares asks for) times
+// 8 / ways over blocks of 16 dimensions; each works relative to its own maximum, and they meet in shared memory.  All shares are
+// asked for at once that way: one warp over twelve shares in turn took 14 us, eight warps over two shares left six of them idle.
 constexpr int JOIN_DIMS = 16, JOIN_WARPS = 8;
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
 attention_tree_merge_rows_kernel(__nv_bfloat16* __restrict__ out, long long o_stride, const TreeArgs a) {
@@ -285,52 +288,72 @@ attention_tree_merge_rows_kernel(__nv_bfloat16* __restrict__ out, long long o_st
     rb::pdl_wait();
     __shared__ float part[JOIN_WARPS][JOIN_DIMS][33], tops[JOIN_WARPS][32], sums[JOIN_WARPS][32];
     const int kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row_blocks = (a.rows_tile + 31) / 32, r0 = blockIdx.x % row_blocks * 32, d0 = blockIdx.x / row_blocks * JOIN_DIMS;
+    const int row_blocks = (a.rows_tile + 31) / 32, r0 = blockIdx.x % row_blocks * 32;
     const int4 note = *note_of(a, kvh, blockIdx.z);
     const int c0 = note.w >> 16, c1 = note.w & 0xffff;
     if (c0 == c1 || r0 >= note.z) return;
-    const int r = min(r0 + lane, note.z - 1);
+    const int r = min(r0 + lane, note.z - 1), n = c1 - c0 + 1;
+    const int ways = n > 8 ? 8 : n > 4 ? 4 : n > 2 ? 2 : 1, chunks = JOIN_WARPS / ways;        // (two shares a warp at a time)
     auto place = [&](int c) { return (size_t)(2 * c + (c == c0 ? 1 : 0)) * a.nkv + kvh; };
-    float top = NEG_BIG, total = 0.f, acc[JOIN_DIMS];
+    const int step = gridDim.x / row_blocks * chunks * JOIN_DIMS;
+    for (int base = blockIdx.x / row_blocks * chunks * JOIN_DIMS; base < a.hd; base += step) {
+        const int d0 = base + warp / ways * JOIN_DIMS;
+        float top = NEG_BIG, total = 0.f, acc[JOIN_DIMS];
 #pragma unroll
-    for (int d = 0; d < JOIN_DIMS; ++d) acc[d] = 0.f;
-#pragma unroll 2
-    for (int c = c0 + warp; c <= c1; c += JOIN_WARPS) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (place(c) * a.rows_tile + r) * 2);
-        const float* src = a.part_o + (place(c) * a.hd + d0) * a.rows_tile + r;
-        float x[JOIN_DIMS];
+        for (int d = 0; d < JOIN_DIMS; ++d) acc[d] = 0.f;
+        if (d0 < a.hd) {
+            for (int c = c0 + warp % ways; c <= c1; c += 2 * ways) {
+                // two shares at a time, all of both asked for before either is used
+                float2 ml[2];
+                float4 x[2][JOIN_DIMS / 4];
 #pragma unroll
-        for (int d = 0; d < JOIN_DIMS; ++d) x[d] = src[(size_t)d * a.rows_tile];
-        const float top_new = fmaxf(top, ml.x), old = exp2f(top - top_new), w = exp2f(ml.x - top_new);
-        top = top_new;
-        total = fmaf(total, old, ml.y * w);
+                for (int i = 0; i < 2; ++i) {
+                    const int ci = min(c + i * ways, c1);
+                    ml[i] = *reinterpret_cast<const float2*>(a.part_ml + (place(ci) * a.rows_tile + r) * 2);
+                    const float4* src = reinterpret_cast<const float4*>(a.part_o + (place(ci) * a.hd + d0) * a.rows_tile) + r;
 #pragma unroll
-        for (int d = 0; d < JOIN_DIMS; ++d) acc[d] = fmaf(acc[d], old, x[d] * w);
+                    for (int d = 0; d < JOIN_DIMS / 4; ++d) x[i][d] = src[d * a.rows_tile];
+                }
+                if (c + ways > c1) ml[1] = make_float2(NEG_BIG, 0.f);
+                const float top_new = fmaxf(top, fmaxf(ml[0].x, ml[1].x)), old = exp2f(top - top_new);
+                const float w0 = exp2f(ml[0].x - top_new), w1 = c + ways > c1 ? 0.f : exp2f(ml[1].x - top_new);
+                top = top_new;
+                total = fmaf(total, old, fmaf(ml[0].y, w0, ml[1].y * w1));
+#pragma unroll
+                for (int d = 0; d < JOIN_DIMS / 4; ++d) {
+                    acc[4 * d] = fmaf(acc[4 * d], old, fmaf(x[0][d].x, w0, x[1][d].x * w1));
+                    acc[4 * d + 1] = fmaf(acc[4 * d + 1], old, fmaf(x[0][d].y, w0, x[1][d].y * w1));
+                    acc[4 * d + 2] = fmaf(acc[4 * d + 2], old, fmaf(x[0][d].z, w0, x[1][d].z * w1));
+                    acc[4 * d + 3] = fmaf(acc[4 * d + 3], old, fmaf(x[0][d].w, w0, x[1][d].w * w1));
+                }
+            }
+        }
+        __syncthreads();
+        tops[warp][lane] = top;
+        sums[warp][lane] = total;
+#pragma unroll
+        for (int d = 0; d < JOIN_DIMS; ++d) part[warp][d][lane] = acc[d];
+        __syncthreads();
+        // two neighbouring dimensions of a row a thread and round
+        for (int i = threadIdx.x; i < chunks * (JOIN_DIMS / 2) * 32; i += 32 * JOIN_WARPS) {
+            const int d = i % (JOIN_DIMS / 2) * 2, rr = i / (JOIN_DIMS / 2) % 32, chunk = i / (JOIN_DIMS / 2 * 32), w0 = chunk * ways;
+            if (r0 + rr >= note.z || base + chunk * JOIN_DIMS >= a.hd) continue;
+            const int row = note.y + r0 + rr, node = row / a.group, head = kvh * a.group + row % a.group;
+            const float sink = (a.sinks ? a.sinks[head] : a.sink) * LOG2E;
+            float m = rb::has_sink(sink) ? sink : NEG_BIG;
+            for (int w = w0; w < w0 + ways; ++w) m = fmaxf(m, tops[w][rr]);
+            float l = rb::has_sink(sink) ? exp2f(sink - m) : 0.f, y0 = 0.f, y1 = 0.f;
+            for (int w = w0; w < w0 + ways; ++w) {
+                const float f = exp2f(tops[w][rr] - m);
+                l = fmaf(sums[w][rr], f, l);
+                y0 = fmaf(part[w][d][rr], f, y0);
+                y1 = fmaf(part[w][d + 1][rr], f, y1);
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            *reinterpret_cast<__nv_bfloat162*>(out + (size_t)(note.x + node) * o_stride + (size_t)head * a.hd + base + chunk * JOIN_DIMS + d) =
+                __floats2bfloat162_rn(y0 * inv, y1 * inv);
+        }
     }
-    tops[warp][lane] = top;
-    sums[warp][lane] = total;
-#pragma unroll
-    for (int d = 0; d < JOIN_DIMS; ++d) part[warp][d][lane] = acc[d];
-    __syncthreads();
-    // a thread two neighbouring dimensions of a row
-    const int rr = threadIdx.x / (JOIN_DIMS / 2), d = threadIdx.x % (JOIN_DIMS / 2) * 2, row = note.y + r0 + rr;
-    static_assert(32 * JOIN_WARPS == 32 * JOIN_DIMS / 2, "a thread two outputs");
-    if (r0 + rr >= note.z) return;
-    const int node = row / a.group, head = kvh * a.group + row % a.group;
-    const float sink = (a.sinks ? a.sinks[head] : a.sink) * LOG2E;
-    float m = rb::has_sink(sink) ? sink : NEG_BIG;
-#pragma unroll
-    for (int w = 0; w < JOIN_WARPS; ++w) m = fmaxf(m, tops[w][rr]);
-    float l = rb::has_sink(sink) ? exp2f(sink - m) : 0.f, y0 = 0.f, y1 = 0.f;
-#pragma unroll
-    for (int w = 0; w < JOIN_WARPS; ++w) {
-        const float f = exp2f(tops[w][rr] - m);
-        l = fmaf(sums[w][rr], f, l);
-        y0 = fmaf(part[w][d][rr], f, y0);
-        y1 = fmaf(part[w][d + 1][rr], f, y1);
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<__nv_bfloat162*>(out + (size_t)(note.x + node) * o_stride + (size_t)head * a.hd + d0 + d) = __floats2bfloat162_rn(y0 * inv, y1 * inv);
 }
 
 template <typename T, int BLOCKS>
@@ -418,7 +441,7 @@ extern "C" int rb_attention_tree(const RbTreeCall* call, void* stream) {
     }
     if (rc != RB_OK || x.shares == 1) return rc;
     if (tc5) {
-        RB_LAUNCH((attention_tree_merge_rows_kernel), dim3((x.rows_tile + 31) / 32 * (x.hd / JOIN_DIMS), x.nkv, a.n_notes), dim3(32 * JOIN_WARPS), 0, st, (__nv_bfloat16*)x.out, x.o_stride, a);
+        RB_LAUNCH((attention_tree_merge_rows_kernel), dim3((x.rows_tile + 31) / 32 * (x.hd / (a.notes_by_unit ? JOIN_DIMS : 64)), x.nkv, a.n_notes), dim3(32 * JOIN_WARPS), 0, st, (__nv_bfloat16*)x.out, x.o_stride, a);
         return RB_OK;
     }
     return x.dtype == RB_F32 ? launch_merge<float>(x.out, x.o_stride, a, st) : launch_merge<__nv_bfloat16>(x.out, x.o_stride, a, st);

@@ -120,10 +120,10 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tmem_relinquish();
     }
     tc_fence_before();
-    prefix_tiles(a, pre, tl);              // (ends with a block-wide barrier)
+    const int extra = prefix_tiles(a, pre, tl);              // (ends with a block-wide barrier)
     tc_fence_after();
     const uint32_t tmem_base = bar->tmem_slot;
-    Pieces pieces(pre, a.B, a.shares, blockIdx.x);
+    Pieces pieces(pre, a.B, a.shares, blockIdx.x, extra);
     int b, mt, p0, p1;
 
     if (warp == 0) {
@@ -131,12 +131,22 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         const int q_bytes = a.rows_tile * 128 * HALVES;
         bool ok = true;
         int it = 0, piece = 0;             // tiles and pieces so far
-        while (ok && pieces.next(pre, tl, b, mt, p0, p1)) {
-            const Seq s = seq_of(a, b);
+        // A piece's lengths and the ids of its first 32 pages are two reads one after the other: they are looked up while the piece before is loaded.
+        Seq s{}, s_next{};
+        int page = 0, page_next = 0, b_next = 0, mt_next = 0, p0_next = 0, p1_next = 0;
+        auto look_ahead = [&]() -> bool {
+            if (!pieces.next(pre, tl, b_next, mt_next, p0_next, p1_next)) return false;
+            s_next = seq_of(a, b_next);
+            page_next = p0_next + lane < p1_next ? a.block_table[(size_t)s_next.slot * a.max_pages + tile_of(s_next, p0_next + lane)] : 0;
+            return true;
+        };
+        bool more = look_ahead();
+        while (ok && more) {
+            s = s_next; page = max(0, page_next); mt = mt_next; p0 = p0_next; p1 = p1_next;
+            more = look_ahead();
             const int* table = a.block_table + (size_t)s.slot * a.max_pages;
-            int page = 0;
             for (int j = p0; j < p1 && ok; ++j, ++it) {
-                if ((j - p0) % 32 == 0) page = j + lane < p1 ? max(0, table[tile_of(s, j + lane)]) : 0;      // 32 pages' ids at a time
+                if (j > p0 && (j - p0) % 32 == 0) page = j + lane < p1 ? max(0, table[tile_of(s, j + lane)]) : 0;      // 32 pages' ids at a time
                 const int row = (__shfl_sync(0xffffffffu, page, (j - p0) & 31) * a.nkv + kvh) * PAGE;
                 const int st = it % STAGES;
                 const uint32_t free_parity = ((it / STAGES) & 1) ^ 1;
@@ -245,6 +255,8 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             const bool row_here = r < rows, warp_here = quarter * 32 < rows;
             const int node = (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
             float m_used = NEG_BIG, l_sum = 0.f;
+            RowBits bits;
+            if (row_here) bits.load(a, s.q0 + node);
             for (int j = p0; j < p1; ++j, ++it) {
                 const int buf = it & 1, st = it % STAGES;
                 const int key0 = tile_of(s, j) * BK;
@@ -253,7 +265,7 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                 unsigned long long seen = ~0ull;
                 bool spoiled = false;
                 if (!whole_tile) {
-                    seen = row_here ? seen_bits(a, s.q0 + node, s.ctx, s.n, key0) : 0ull;
+                    seen = row_here ? bits.seen(a, s.ctx, s.n, key0) : 0ull;
                     // Weights of zero still multiply what lies in V: rows past the sequence's end are stale, and a value that is not finite
                     // must not reach a row that does not see it.  Such values become zero here, and the rows that do see them NaN.
                     alive = __all_sync(0xffffffffu, wait_or_abort(&bar->v_full[st], (it / STAGES) & 1, &bar->abort_flag));
@@ -266,14 +278,19 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                         uint4* at = reinterpret_cast<uint4*>(Vt + (ch >> 3) * KV_HALF + vr * 128 + (((ch & 7) ^ (vr & 7)) << 4));
                         if (vr >= valid) { *at = make_uint4(0, 0, 0, 0); continue; }
                         uint4 x = *at;
-                        uint32_t* w = &x.x;
-                        bool bad = false;
+                        // (an exponent of all ones carries into the sign's place)
+                        const uint32_t carry = ((x.x & 0x7f807f80u) + 0x00800080u) | ((x.y & 0x7f807f80u) + 0x00800080u) |
+                                               ((x.z & 0x7f807f80u) + 0x00800080u) | ((x.w & 0x7f807f80u) + 0x00800080u);
+                        if (carry & 0x80008000u) {
+                            uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if ((w[e] & 0x7f80u) == 0x7f80u) { w[e] &= 0xffff0000u; bad = true; }
-                            if ((w[e] & 0x7f800000u) == 0x7f800000u) { w[e] &= 0xffffu; bad = true; }
+                            for (int e = 0; e < 4; ++e) {
+                                if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
+                                if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu;
+                            }
+                            *at = make_uint4(w[0], w[1], w[2], w[3]);
+                            atomicOr(&bar->bad[checks % 3][vr >> 5], 1u << (vr & 31));
                         }
-                        if (bad) { *at = x; atomicOr(&bar->bad[checks % 3][vr >> 5], 1u << (vr & 31)); }
                     }
                     fence_proxy_async();
                     // Three words of flags in turn: those of the next masked tile are cleared by a thread that has seen everybody arrive at the one before
@@ -366,28 +383,30 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                     if (rb::has_sink(sink)) l_sum += exp2f(fminf(sink - m_used, 126.f));
                 }
                 const float f = !whole ? 1.f : l_sum == 0.f ? 0.f : 1.f / l_sum;
-                // (a place's result is [HD][rows]: a warp writes 32 rows of a dimension as one line)
+                // (a place's result is [HD / 4][rows][4]: a warp writes 32 rows' 16 bytes side by side)
                 const size_t place = (size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * a.nkv + kvh;
                 __nv_bfloat16* orow = out + (size_t)(s.q0 + node) * o_stride + (size_t)head * HD;
-                float* prow = a.part_o + place * HD * a.rows_tile + r;
+                float* prow = a.part_o + place * HD * a.rows_tile + r * 4;
                 if (!whole && row_here) *reinterpret_cast<float2*>(a.part_ml + (place * a.rows_tile + r) * 2) = make_float2(m_used, l_sum);
 #pragma unroll 1
-                for (int c = 0; c < HD / 16; ++c) {
-                    float ov[16];
-                    tmem_ld16(lane_base + 2 * BK + c * 16, ov);
+                for (int c = 0; c < HD / 64; ++c) {
+                    float ov[64];
+                    tmem_ld64(lane_base + 2 * BK + c * 64, ov);
                     if (!row_here) continue;
                     if (whole) {
-                        uint32_t w[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            __nv_bfloat162 h = __floats2bfloat162_rn(ov[2 * i] * f, ov[2 * i + 1] * f);
-                            w[i] = *reinterpret_cast<uint32_t*>(&h);
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(ov[8 * i + 2 * e] * f, ov[8 * i + 2 * e + 1] * f);
+                                w[e] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                            reinterpret_cast<uint4*>(orow + c * 64)[i] = make_uint4(w[0], w[1], w[2], w[3]);
                         }
-                        reinterpret_cast<uint4*>(orow + c * 16)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                        reinterpret_cast<uint4*>(orow + c * 16)[1] = make_uint4(w[4], w[5], w[6], w[7]);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) prow[(size_t)(c * 16 + i) * a.rows_tile] = ov[i];
+                        for (int i = 0; i < 16; ++i) rb::store4(prow + (size_t)(c * 16 + i) * a.rows_tile * 4, ov + 4 * i);
                     }
                 }
             }

@@ -42,33 +42,49 @@ __device__ __forceinline__ Seq seq_of(const TreeArgs& a, int b) {
 }
 __device__ __forceinline__ int tile_of(const Seq& s, int j) { return j < s.kept ? j : s.first + (j - s.kept); }
 
-// pre[b] = (tile of keys, tile of rows) pairs of the sequences before b, pre[B] = all of them; tl[b] = tiles of keys of sequence b.  Every thread
-// of the block calls this.
-__device__ __forceinline__ void prefix_tiles(const TreeArgs& a, int* pre, int* tl) {
+// What a block pays for beginning and ending a (sequence, tile of rows), and for the masked tiles at its ends, in tiles of keys: each counts as so
+// many tiles more when the work is shared out, a third of a share at most.  (Eight sequences of 900 to 9,000 keys under a window of 4,096, 12
+// tiles a block: blocks with two pieces took 28 us where those with one took 20.)
+constexpr int MAX_EXTRA = 4;
+
+// The work of a key/value head, laid end to end: pre[b] = tiles of keys times tiles of rows of the sequences before b, pre[B] = of all of them, with
+// `extra` (returned) more of keys each; tl[b] = tiles of keys of sequence b, with as many more (0: nothing to do).  Every thread of the block calls
+// this.
+__device__ __forceinline__ int prefix_tiles(const TreeArgs& a, int* pre, int* tl) {
     for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
         const Seq s = seq_of(a, b);
-        tl[b] = s.tiles;
         pre[b + 1] = s.tiles * s.units;
+        tl[b] = s.units;
     }
     if (threadIdx.x == 0) pre[0] = 0;
     __syncthreads();
     if (a.B > 1) {
         if (threadIdx.x < 32) {
-            int carry = 0;
+            int pairs = 0, units = 0;                      // of the sequences before b0
             for (int b0 = 0; b0 < a.B; b0 += 32) {
                 const int b = b0 + threadIdx.x;
-                int v = b < a.B ? pre[b + 1] : 0;
+                int v = b < a.B ? pre[b + 1] : 0, u = b < a.B ? tl[b] : 0;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const int u = __shfl_up_sync(0xffffffffu, v, o);
-                    if ((int)threadIdx.x >= o) v += u;
+                    const int v2 = __shfl_up_sync(0xffffffffu, v, o), u2 = __shfl_up_sync(0xffffffffu, u, o);
+                    if ((int)threadIdx.x >= o) { v += v2; u += u2; }
                 }
-                if (b < a.B) pre[b + 1] = carry + v;
-                carry += __shfl_sync(0xffffffffu, v, 31);
+                if (b < a.B) { pre[b + 1] = pairs + v; tl[b] = units + u; }
+                pairs += __shfl_sync(0xffffffffu, v, 31);
+                units += __shfl_sync(0xffffffffu, u, 31);
             }
         }
         __syncthreads();
     }
+    const int extra = min(MAX_EXTRA, pre[a.B] / (3 * a.shares));
+    __syncthreads();
+    for (int b = threadIdx.x; b < a.B; b += blockDim.x) {
+        const int t = seq_of(a, b).tiles;
+        pre[b + 1] += extra * tl[b];
+        tl[b] = t > 0 ? t + extra : 0;
+    }
+    __syncthreads();
+    return extra;
 }
 // The sequence that holds pair f (f < pre[B]).
 __device__ __forceinline__ int sequence_of(const int* pre, int B, int f) {
@@ -82,25 +98,32 @@ __device__ __forceinline__ int sequence_of(const int* pre, int B, int f) {
 
 // Walks the pieces that one share holds: of a sequence's tiles of rows one after the other, each over all its tiles of keys.
 struct Pieces {
-    int f, end, b, W, shares;
-    __device__ Pieces(const int* pre, int B, int n_shares, int c) {
+    int f, end, b, W, shares, extra, begin;      // begin: where the last piece's (sequence, tile of rows) begins
+    __device__ Pieces(const int* pre, int B, int n_shares, int c, int more) : extra(more) {
         W = pre[B];
         shares = max(1, min(n_shares, W));           // (no share between two others is empty: joining counts on it)
-        f = c < shares ? (int)((long long)c * W / shares) : 0;
-        end = c < shares ? (int)((c + 1ll) * W / shares) : 0;
+        // (64-bit divisions take half a microsecond)
+        const bool small = W < 0x7fffffff / (shares + 1);
+        f = c >= shares ? 0 : small ? c * W / shares : (int)((long long)c * W / shares);
+        end = c >= shares ? 0 : small ? (c + 1) * W / shares : (int)((c + 1ll) * W / shares);
         b = sequence_of(pre, B, f);
     }
     // the next piece: tiles of keys [p0, p1) for tile of rows mt of sequence `seq`; false: none is left
     __device__ bool next(const int* pre, const int* tl, int& seq, int& mt, int& p0, int& p1) {
-        if (f >= end) return false;
-        while (pre[b + 1] <= f) ++b;
-        seq = b;
-        const int t = tl[b], off = f - pre[b];
-        mt = off / t;
-        p0 = off - mt * t;
-        p1 = min(t, p0 + end - f);
-        f += p1 - p0;
-        return true;
+        for (;;) {
+            if (f >= end) return false;
+            while (pre[b + 1] <= f) ++b;
+            const int t = tl[b], off = f - pre[b];
+            mt = off / t;
+            p0 = off - mt * t;
+            begin = f - p0;
+            const int stop = min(t, p0 + end - f);
+            f += stop - p0;
+            if (p0 >= t - extra) continue;            // nothing but what is counted on top
+            seq = b;
+            p1 = min(stop, t - extra);
+            return true;
+        }
     }
     // the share that holds pair g: the last c with c W / shares <= g
     __device__ int share_of(int g) const { return (int)(((g + 1ll) * shares - 1) / W); }
@@ -112,7 +135,7 @@ __device__ __forceinline__ int4* note_of(const TreeArgs& a, int kvh, int entry) 
 // One thread of a block calls this for every piece.
 __device__ __forceinline__ void note_piece(const TreeArgs& a, const Pieces& p, const Seq& s, int kvh, int c, int b, int mt, int p0, int p1) {
     if (p0 != 0) return;
-    const int last = p1 == s.tiles ? c : p.share_of(p.f - p1 + s.tiles - 1);
+    const int last = p1 == s.tiles ? c : p.share_of(p.begin + s.tiles - 1);
     const int row0 = mt * a.rows_tile;
     const int4 note = make_int4(s.q0, row0, min(a.rows_tile, s.n * a.group - row0), (c << 16) | last);
     if (a.notes_by_unit) *note_of(a, kvh, b * a.max_units + mt) = note;
@@ -129,12 +152,12 @@ __device__ __forceinline__ void note_nothing(const TreeArgs& a, const Pieces& p,
             }
         return;
     }
-    // by shares: this one has an entry unless its end cuts what began in it
+    // by shares: this one has an entry if its end cuts the tiles of what began in it
     if (tid == 0 && c < a.n_notes) {
         bool cuts = false;
         if (c + 1 < p.shares && p.f < p.end) {
-            const int b = sequence_of(pre, a.B, p.end), begin = p.end - (p.end - pre[b]) % tl[b];
-            cuts = begin != p.end && begin >= p.f;
+            const int b = sequence_of(pre, a.B, p.end), into = (p.end - pre[b]) % tl[b];
+            cuts = into != 0 && into < tl[b] - p.extra && p.end - into >= p.f;
         }
         if (!cuts) *note_of(a, kvh, c) = none;
     }
@@ -148,26 +171,38 @@ __device__ __forceinline__ unsigned long long range_bits(int a, int b) {
     const unsigned long long upto = b == 64 ? ~0ull : (1ull << b) - 1ull;
     return upto & ~((1ull << a) - 1ull);
 }
-// Which of the 64 keys from key0 on row `t` (a node of a sequence with context ctx and n nodes) sees.
-__device__ __forceinline__ unsigned long long seen_bits(const TreeArgs& a, int t, int ctx, int n, int key0) {
-    unsigned long long m = range_bits(0, ctx - key0);
-    if (a.window > 0 && m) {
-        const int lo = a.positions[t] - a.window + 1;
-        m &= range_bits(lo - key0, 64) | range_bits(0, a.keep - key0);
-    }
-    const int off = key0 - ctx;                       // the node at the tile's first key
-    if (off + 64 > 0 && off < n) {
-        const int* row = a.visible + (size_t)t * a.words;
-        const int w0 = off >> 5;                      // (rounds down below zero too)
-        const int sh = off & 31;
-        unsigned int w[3];
+// A row's words of bits, and its position, read once a piece.
+constexpr int MAX_WORDS = 8;
+struct RowBits {
+    unsigned int w[MAX_WORDS];
+    int position;
+    __device__ void load(const TreeArgs& a, int t) {
 #pragma unroll
-        for (int i = 0; i < 3; ++i) w[i] = (w0 + i >= 0 && w0 + i < a.words) ? (unsigned int)row[w0 + i] : 0u;
-        const unsigned int lo = __funnelshift_r(w[0], w[1], sh), hi = __funnelshift_r(w[1], w[2], sh);
-        m |= (((unsigned long long)hi << 32) | lo) & range_bits(-off, n - off);
+        for (int i = 0; i < MAX_WORDS; ++i) w[i] = i < a.words ? (unsigned int)a.visible[(size_t)t * a.words + i] : 0u;
+        position = a.window > 0 ? a.positions[t] : 0;
     }
-    return m;
-}
+    // Which of the 64 keys from key0 on the row (a node of a sequence with context ctx and n nodes) sees.
+    __device__ unsigned long long seen(const TreeArgs& a, int ctx, int n, int key0) const {
+        unsigned long long m = range_bits(0, ctx - key0);
+        if (a.window > 0 && m) {
+            const int lo = position - a.window + 1;
+            m &= range_bits(lo - key0, 64) | range_bits(0, a.keep - key0);
+        }
+        const int off = key0 - ctx;                       // the node at the tile's first key
+        if (off + 64 > 0 && off < n) {
+            const int w0 = off >> 5, sh = off & 31;       // (rounds down below zero too)
+            unsigned int x[3] = {0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < MAX_WORDS; ++i) {
+#pragma unroll
+                for (int j = 0; j < 3; ++j) x[j] = i == w0 + j ? w[i] : x[j];
+            }
+            const unsigned int lo = __funnelshift_r(x[0], x[1], sh), hi = __funnelshift_r(x[1], x[2], sh);
+            m |= (((unsigned long long)hi << 32) | lo) & range_bits(-off, n - off);
+        }
+        return m;
+    }
+};
 
 // attention_tree_tc5.cu: bfloat16, head sizes 64, 128 and 256; rows_tile = 128 / group * group.
 int launch_tc5(const void* q, long long q_stride, int T, void* out, long long o_stride, const void* k, const void* v, int n_pages,

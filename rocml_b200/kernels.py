@@ -930,10 +930,12 @@ def _tree_sizes(what: str, visible, cu_q, n_seqs: int, max_nodes: int):
 _TREE_CALL = struct.Struct("@13P2q14i3f")
 
 
-def tree_shares(pairs: int, nkv: int, slots: int) -> int:
-    """How many blocks a key/value head's work is shared among (csrc/attention_tree.cu): as many as fill the device once over all heads, never
-    more than there are (page, tile of rows) pairs; with more heads than blocks run at once, about four waves of blocks."""
-    return max(1, min(slots // nkv if nkv <= slots else -(-4 * slots // nkv), pairs))
+def tree_shares(pairs: int, rows: int, nkv: int, slots: int) -> int:
+    """How many blocks a key/value head's work, ``pairs`` (page, tile of rows) pairs, is shared among (csrc/attention_tree.cu): as many as fill the
+    device once over all heads (with more heads than blocks run at once, about four waves of them), but at least a page a block for every
+    sixteen of a tile's ``rows``: what a block leaves to be joined is as much as that to write and read again.  (256 rows over 4,164 keys, 8 heads,
+    in blocks of 3.5 pages 21.5 us, of 8 pages 18.5; 16 rows over 709 keys in blocks of one page 10.7, of two 11.6.)"""
+    return max(1, min(slots // nkv if nkv <= slots else -(-4 * slots // nkv), pairs // max(1, rows // 16)))
 
 
 @_profiled(lambda a, facts: _attention_cost(a, facts))
@@ -947,7 +949,7 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     those whose bit is set in its row of ``visible`` (int32 [T, words], bit j % 32 of word j / 32): its ancestors and itself, as a rule.
     ``window`` > 0: of the context only the places above positions[t] - window (``positions`` int32 [T], none below kv_len - n), and those below
     ``keep``.  ``sink`` and ``softcap`` as in ``attention_generic``.  ``max_kv_len``: the longest sequence, if known (it decides how the work is
-    split, nothing else).  A row that sees nothing is zero.  Rows of slots below 0, of sequences shorter than their tree or longer than their row of the block
+    split, and with that the order of 32-bit sums, nothing else).  A row that sees nothing is zero.  Rows of slots below 0, of sequences shorter than their tree or longer than their row of the block
     table stay as they are.  What a row does not see takes no part in its result, whatever it holds; a bfloat16 row that sees a value
     that is not finite may become NaN as a whole."""
     tokens, words = _tree_sizes("attention_tree", visible, cu_q, n_seqs, max_nodes)
@@ -984,7 +986,7 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         rows_tile = 128 // group * group               # the tensor-core kernel: whole nodes in 128 rows
         slots = slots // 3 * (2 if hd <= 128 else 1)
     units = n_seqs * -(-max_nodes * group // rows_tile)
-    shares = tree_shares(longest * units, nkv, slots)
+    shares = tree_shares(longest * units, min(rows_tile, max_nodes * group), nkv, slots)
     work = None
     if shares > 1:
         work = torch.empty(2 * shares * nkv * rows_tile * (hd + 2) + 4 * nkv * min(shares - 1, units), dtype=torch.float32, device=device)

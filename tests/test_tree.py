@@ -9,24 +9,26 @@ from rocml_b200 import kernels
 from rocml_b200.errors import KernelError
 
 
-def pieces_of(sizes, shares):
+def pieces_of(sizes, n_shares):
     """What csrc/attention_tree.cu's blocks do with sequences of so many (tiles of keys, tiles of rows): {share: [(sequence, tile of rows, first, end)]}."""
+    extra = min(4, sum(t * u for t, u in sizes) // (3 * n_shares))
     pre = [0]
     for t, u in sizes:
-        pre.append(pre[-1] + t * u)
-    out, shares = {}, max(1, min(shares, pre[-1]))
+        pre.append(pre[-1] + ((t + extra) * u if t else 0))
+    out, shares = {}, max(1, min(n_shares, pre[-1]))
     for c in range(shares):
         f, end = c * pre[-1] // shares, (c + 1) * pre[-1] // shares
         b, got = sequence_of(pre, f), []
         while f < end:
             while pre[b + 1] <= f:
                 b += 1
-            mt, p0 = divmod(f - pre[b], sizes[b][0])
-            p1 = min(sizes[b][0], p0 + end - f)
-            got.append((b, mt, p0, p1))
-            f += p1 - p0
+            mt, p0 = divmod(f - pre[b], sizes[b][0] + extra)
+            stop = min(sizes[b][0] + extra, p0 + end - f)
+            f += stop - p0
+            if p0 < sizes[b][0]:
+                got.append((b, mt, p0, min(stop, sizes[b][0])))
         out[c] = got
-    return pre, out, shares
+    return pre, out, shares, extra
 
 
 def sequence_of(pre, f):
@@ -42,7 +44,7 @@ def test_shares_cover_every_tile_once_and_pieces_have_places_of_their_own(seed):
     rng = random.Random(seed)
     sizes = [(t, rng.choice([1, 1, 2, 5]) if t else 0) for t in [rng.choice([0, 1, 2, 3, rng.randrange(1, 200)]) for _ in range(rng.randrange(1, 40))]]
     shares = rng.choice([1, 2, 3, 17, 18, 37, 296])
-    pre, pieces, shares = pieces_of(sizes, shares)
+    pre, pieces, shares, extra = pieces_of(sizes, shares)
     W = pre[-1]
     seen, places = {}, {}
     for c, got in pieces.items():
@@ -64,7 +66,7 @@ def test_shares_cover_every_tile_once_and_pieces_have_places_of_their_own(seed):
         f, end = c * W // shares, (c + 1) * W // shares
         for b, mt, p0, p1 in got:
             if p0 == 0:
-                last = c if p1 == sizes[b][0] else share_of(pre[b] + mt * sizes[b][0] + sizes[b][0] - 1)
+                last = c if p1 == sizes[b][0] else share_of(pre[b] + mt * (sizes[b][0] + extra) + sizes[b][0] - 1)
                 assert (b, mt) not in by_unit
                 by_unit[b, mt] = (c, last)
                 if last != c:
@@ -73,8 +75,8 @@ def test_shares_cover_every_tile_once_and_pieces_have_places_of_their_own(seed):
         cuts = False
         if c + 1 < shares and f < end:
             b = sequence_of(pre, end)
-            begin = end - (end - pre[b]) % sizes[b][0]
-            cuts = begin != end and begin >= f
+            into = (end - pre[b]) % (sizes[b][0] + extra)
+            cuts = 0 < into < sizes[b][0] and end - into >= f
         assert cuts == (c in by_share)
     for (b, mt), (c0, c1) in by_unit.items():
         for c in range(c0, c1 + 1) if c0 != c1 else ():
@@ -121,10 +123,11 @@ def test_confirmed_nodes_by_bits_are_the_walk(seed):
 
 
 def test_shares_fill_the_device_and_never_outnumber_the_pages():
-    assert kernels.tree_shares(200, 8, 296) == 37
-    assert kernels.tree_shares(3, 8, 296) == 3
-    assert kernels.tree_shares(320, 1000, 296) == 2
-    assert kernels.tree_shares(1, 5000, 296) == 1
+    assert kernels.tree_shares(200, 64, 8, 296) == 37
+    assert kernels.tree_shares(200, 128, 8, 296) == 25
+    assert kernels.tree_shares(3, 16, 8, 296) == 3
+    assert kernels.tree_shares(320, 5, 1000, 296) == 2
+    assert kernels.tree_shares(1, 128, 5000, 296) == 1
 
 
 def _attention(**change):

@@ -128,18 +128,20 @@ def test_attention_tree_hidden_places_may_hold_anything(dtype, hd):
 @pytest.mark.parametrize("dtype,hd", [(torch.float32, 64), (torch.bfloat16, 128)])
 def test_attention_tree_leaves_other_rows_alone(dtype, hd):
     """Padding sequences (slot -1, no rows), sequences that say less than their tree or more than their row of the table, rows behind the
-    last sequence: nothing is written there, and the others are what they were."""
+    last sequence: nothing is written there, and the others are right.  (Not the same bits: where a sequence's keys are cut among blocks depends on
+    the other sequences, and the order of 32-bit sums on that.)"""
     t = Trees(8, [(100, 4), (50, 6), (30, 3), (20, 2)], 4, 2, hd, dtype)
-    want = call(t)
+    want, mass = plain_tree.attention(t, hd ** -0.5)
+    right = lambda out, n: ((out[:n].double().cpu() - want[:n]).abs() <= bound(want, mass, dtype, hd in (64, 128, 256))[:n]).all()
     slots, lens = list(t.slots), [c + n for c, n in t.sizes]
     slots[1] = -1
     lens[2] = 2
     lens[3] = 64 * t.table.shape[1] + 1
     i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
     out = call(t, seq_slot=i32(slots), kv_len=i32(lens))
-    assert torch.equal(out[:4], want[:4]) and (out[4:] == 7.0).all()
+    assert right(out, 4) and (out[4:] == 7.0).all()
     out = call(t, cu_q=i32([0, 4, 10, 10, 10]))          # the last two bring nothing
-    assert torch.equal(out[:10], want[:10]) and (out[10:] == 7.0).all()
+    assert right(out, 10) and (out[10:] == 7.0).all()
 
 
 @pytest.mark.parametrize("dtype,hd", [(torch.float32, 48), (torch.bfloat16, 128), (torch.bfloat16, 64)])
@@ -155,7 +157,7 @@ def test_attention_tree_strided_rows(dtype, hd):
         out = torch.full_like(q, 7.0)
         q[:, left:left + W] = t.q.to(DEV)
         kernels.attention_tree(q[:, left:left + W], out[:, left:left + W], t.k[0].to(DEV), t.v[0].to(DEV), d["block_table"], d["seq_slot"],
-                               d["cu_q"], d["kv_len"], d["visible"], 2, 21, 4, 2, hd, hd ** -0.5)
+                               d["cu_q"], d["kv_len"], d["visible"], 2, 21, 4, 2, hd, hd ** -0.5, max_kv_len=354)
         kernels.check_status(DEV)
         check(t, dtype, out[:, left:left + W])
         if left == 8:
@@ -221,7 +223,8 @@ def test_attention_tree_behind_32_bit_offsets():
     for p in set(int(x) for x in t.table.reshape(-1) if x >= 0):
         k[pages - 1 - p], v[pages - 1 - p] = t.k[0, p].to(DEV), t.v[0, p].to(DEV)
     out = torch.zeros_like(want)
-    kernels.attention_tree(t.q.to(DEV), out, k, v, moved.to(DEV), d["seq_slot"], d["cu_q"], d["kv_len"], d["visible"], 1, 8, 4, 2, 128, 128 ** -0.5)
+    kernels.attention_tree(t.q.to(DEV), out, k, v, moved.to(DEV), d["seq_slot"], d["cu_q"], d["kv_len"], d["visible"], 1, 8, 4, 2, 128, 128 ** -0.5,
+                           max_kv_len=108)
     assert torch.equal(out, want)
 
 
