@@ -26,28 +26,50 @@ using namespace rb_tree;
 
 namespace {
 // ---- any head size, both types, 32-bit multiply-adds ------------------------------------------------------------------
-// 128 threads, 16 rows by 64 keys a tile, keys and values staged 64 dimensions at a time as float32.  Thread (rg, kg), rg = t / 16, kg = t % 16,
-// forms the scores of rows 2 rg, 2 rg + 1 against keys kg + 16 i, and the results of the same rows at dimensions 4 kg .. 4 kg + 3
-// of every block of 64: six 16-byte reads of shared memory for 32 multiply-adds in both products.
+// 128 threads, 16 rows by 64 keys a tile.  Keys and values come 64 dimensions at a time, as float32, through a ring of RING blocks of shared memory:
+// a tile is its blocks of keys, then its blocks of values, and RING - 1 blocks are asked for ahead of the one in use (32-bit rows by cp.async; staged through
+// registers a block waited for memory four times a tile: 10 us).  Thread (rg, kg), rg = t / 16, kg = t % 16, forms the scores of rows 2 rg, 2 rg + 1
+// against keys kg + 16 i, and the results of the same rows at dimensions 4 kg .. 4 kg + 3 of every block of 64: six 16-byte reads of shared
+// memory for 32 multiply-adds in both products.
 constexpr int SR = 16, SLD = 68;      // rows a tile; row stride of a staged [64][64] block (68 floats: 16-byte reads of 8 rows miss each other's banks)
+constexpr int RING = 4;
 
+__device__ __forceinline__ void copy_async16(void* dst, const void* src, bool real) {
+    const unsigned int at = (unsigned int)__cvta_generic_to_shared(dst);
+    const int bytes = real ? 16 : 0;                   // (the rest is zeros)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(src), "r"(bytes) : "memory");
+}
+// [64 keys][64 dims from d0] of a page of this head; rows beyond `rows` and dimensions beyond hd are zero
 template <typename T>
 __device__ __forceinline__ void stage64(const T* src, int hd, int d0, int rows, float* dst) {
-    // [64 keys][64 dims from d0] of a page of this head; rows beyond `rows` and dimensions beyond hd are zero
-    for (int i = threadIdx.x; i < 64 * 16; i += 128) {
-        const int r = i >> 4, d = (i & 15) * 4;
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
+    const int d = (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
+    if (sizeof(T) == 4 && hd % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = r0 + 8 * i;
+            const bool real = r < rows && d0 + d < hd;
+            copy_async16(dst + r * SLD + d, real ? src + (size_t)r * hd + d0 + d : src, real);
+        }
+        return;
+    }
+    float x[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = r0 + 8 * i;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
         if (r < rows) {
             if (hd % 4 == 0) {
-                if (d0 + d < hd) rb::load4(src + (size_t)r * hd + d0 + d, x);
+                if (d0 + d < hd) rb::load4(src + (size_t)r * hd + d0 + d, x[i]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (d0 + d + e < hd) x[e] = rb::to_f32(src[(size_t)r * hd + d0 + d + e]);
+                    if (d0 + d + e < hd) x[i][e] = rb::to_f32(src[(size_t)r * hd + d0 + d + e]);
             }
         }
-        rb::store4(dst + r * SLD + d, x);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rb::store4(dst + (r0 + 8 * i) * SLD + d, x[i]);
 }
 
 template <typename T, int BLOCKS>       // BLOCKS: blocks of 64 dimensions a head, 1, 2, 4 or 8
@@ -58,9 +80,8 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
     rb::pdl_wait();
     extern __shared__ float smem[];
     float* Qs = smem;                              // [16][64 BLOCKS]
-    float* Ks = Qs + SR * 64 * BLOCKS;             // [64][SLD]
-    float* Vs = Ks + 64 * SLD;
-    float* Ps = Vs + 64 * SLD;                     // [16][SLD]
+    float* Ring = Qs + SR * 64 * BLOCKS;           // [RING][64][SLD]
+    float* Ps = Ring + RING * 64 * SLD;            // [16][SLD]
     int* pre = (int*)(Ps + SR * SLD);
     int* tl = pre + a.B + 1;
     const int kvh = blockIdx.y;
@@ -76,13 +97,33 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
         if (a.n_notes && threadIdx.x == 0) note_piece(a, pieces, s, kvh, blockIdx.x, b, mt, p0, p1);
         const int row0 = mt * a.rows_tile, rows = min(SR, s.n * a.group - row0);
         const int* table = a.block_table + (size_t)s.slot * a.max_pages;
+        const int n_blocks = (p1 - p0) * 2 * BLOCKS;
+        // block i of the piece: tile p0 + i / (2 BLOCKS), keys before values
+        auto fetch = [&](int i) {
+            if (i < n_blocks) {
+                const int key0 = tile_of(s, p0 + i / (2 * BLOCKS)) * PAGE, c = i % (2 * BLOCKS);
+                const size_t at = ((size_t)max(0, table[key0 / PAGE]) * a.nkv + kvh) * PAGE * a.hd;
+                stage64((c < BLOCKS ? k_cache : v_cache) + at, a.hd, c % BLOCKS * 64, min(PAGE, s.len - key0), Ring + i % RING * 64 * SLD);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        // the next block has landed, and the one before it is free for what comes RING - 1 blocks later
+        auto arrive = [&](int i) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory");
+            __syncthreads();
+            fetch(i + RING - 1);
+            return Ring + i % RING * 64 * SLD;
+        };
         __syncthreads();
+#pragma unroll 1
+        for (int i = 0; i < RING - 1; ++i) fetch(i);
+#pragma unroll 8
         for (int i = threadIdx.x; i < SR * 64 * BLOCKS; i += 128) {
             const int r = i / (64 * BLOCKS), d = i % (64 * BLOCKS);
             float x = 0.f;
             if (r < rows && d < a.hd) {
-                const int node = (row0 + r) / a.group, h = (row0 + r) % a.group;
-                x = rb::to_f32(q[(size_t)(s.q0 + node) * q_stride + (size_t)(kvh * a.group + h) * a.hd + d]);
+                const int node = (row0 + r) / a.group, h = (row0 + r) - node * a.group;
+                x = rb::to_f32(__ldg(q + (size_t)(s.q0 + node) * q_stride + (size_t)(kvh * a.group + h) * a.hd + d));
             }
             Qs[i] = x;
         }
@@ -97,16 +138,13 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
             for (int r = 0; r < 2; ++r)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[c][r][e] = 0.f;
+        int block = 0;
         for (int j = p0; j < p1; ++j) {
-            const int key0 = tile_of(s, j) * PAGE, valid = min(PAGE, s.len - key0);
-            const int page = max(0, table[key0 / PAGE]);
-            const size_t at = ((size_t)page * a.nkv + kvh) * PAGE * a.hd;
+            const int key0 = tile_of(s, j) * PAGE;
             float sc[2][4] = {};
 #pragma unroll 1
             for (int c = 0; c < BLOCKS; ++c) {
-                __syncthreads();
-                stage64(k_cache + at, a.hd, c * 64, valid, Ks);
-                __syncthreads();
+                const float* Ks = arrive(block++);
 #pragma unroll 4
                 for (int d = 0; d < 64; d += 4) {
                     float qa[2][4], kb[4][4];
@@ -151,9 +189,7 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
             }
 #pragma unroll
             for (int c = 0; c < BLOCKS; ++c) {
-                __syncthreads();
-                stage64(v_cache + at, a.hd, c * 64, valid, Vs);
-                __syncthreads();
+                const float* Vs = arrive(block++);          // (its barrier also makes Ps whole)
 #pragma unroll 4
                 for (int key = 0; key < 64; key += 4) {
                     float pa[2][4], vb[4][4];
@@ -172,6 +208,7 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
                 }
             }
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         const bool whole = p0 == 0 && p1 == s.tiles;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -359,7 +396,7 @@ attention_tree_merge_rows_kernel(__nv_bfloat16* __restrict__ out, long long o_st
 template <typename T, int BLOCKS>
 int launch_simple(const void* q, long long q_stride, void* out, long long o_stride, const void* k, const void* v, const TreeArgs& a,
                   cudaStream_t stream) {
-    const size_t smem = (SR * 64 * BLOCKS + 2 * 64 * SLD + SR * SLD) * sizeof(float) + (2 * a.B + 1) * sizeof(int);
+    const size_t smem = (SR * 64 * BLOCKS + RING * 64 * SLD + SR * SLD) * sizeof(float) + (2 * a.B + 1) * sizeof(int);
     auto kernel = attention_tree_simple_kernel<T, BLOCKS>;
     static rb::PerDevice<int> allowed;
     int device;
@@ -368,7 +405,7 @@ int launch_simple(const void* q, long long q_stride, void* out, long long o_stri
     const int* known;
     const int rc = allowed.get(device, &known, [&](int& x) {
         x = 1;
-        return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
+        return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
     });
     if (rc) return rc;
     RB_LAUNCH((kernel), dim3(a.shares, a.nkv), dim3(128), smem, stream, (const T*)q, q_stride, (T*)out, o_stride, (const T*)k, (const T*)v, a);

@@ -8,7 +8,7 @@
 // The k most likely, largest first, equal ones by their index.  Beside its triple a thread keeps its largest element (and that
 // element's chunk).  All of the k largest elements belong to the k threads whose largest elements lead: any other thread is
 // behind k elements already.  So one pass over the row is enough; afterwards only those k threads' elements (k / threads of the
-// row) are read again.  Keys are 64-bit whole numbers that order like (value, -index), sorted in registers of a warp, 32 at a time.
+// row) are read again, all at once.  Keys are 64-bit whole numbers that order like (value, -index); places are found by counting the keys ahead.
 //
 // A row is read by one block or by the blocks of a cluster, which meet in the first one's shared memory.
 #include "common.cuh"
@@ -21,7 +21,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 // Back from base 2 with the very factor that the logits were multiplied by: a 32-bit log2 e is 2^-25 off, which times a logit of 30 would be seen.
 constexpr double FROM_LOG2 = 1.0 / (double)LOG2E;
 constexpr float NEG_BIG = -1e30f;
-constexpr int THREADS = 512, WARPS = THREADS / 32, MAX_TOP = 32;
+constexpr int THREADS = 256, WARPS = THREADS / 32, MAX_TOP = 32, MAX_BLOCKS = 16;
+constexpr int UNROLL = 4;          // chunks of 32 bytes that a thread has asked for at once
 typedef unsigned long long Key;
 
 // Orders like (x, -index); larger first.  Zero is below every key of an element.
@@ -76,21 +77,27 @@ __device__ __forceinline__ Sum join(Sum a, Sum b) {
 }
 
 template <typename T> struct Chunk;                  // 32 bytes
-template <> struct Chunk<float> { static constexpr int E = 8; };
-template <> struct Chunk<__nv_bfloat16> { static constexpr int E = 16; };
+// (sixteen values a chunk take more registers: three blocks a multiprocessor instead of four, or they spill)
+template <> struct Chunk<float> { static constexpr int E = 8, BLOCKS_PER_SM = 4; };
+template <> struct Chunk<__nv_bfloat16> { static constexpr int E = 16, BLOCKS_PER_SM = 3; };
 
+// Eight words as they lie in memory -> E values.
+template <typename T>
+__device__ __forceinline__ void unpack_chunk(const uint4& a, const uint4& b, float* x) {
+    const unsigned int w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (Chunk<T>::E == 8) x[i] = __uint_as_float(w[i]);
+        else { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+}
 // The chunk whose first element is `i0` (which may lie before the row, or end after it: -inf there).
 template <typename T>
 __device__ __forceinline__ void load_chunk(const T* row, int i0, int V, float* x) {
     constexpr int E = Chunk<T>::E;
     if (i0 >= 0 && i0 + E <= V) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + i0)), b = __ldg(reinterpret_cast<const uint4*>(row + i0) + 1);
-        const unsigned int w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (E == 8) x[i] = __uint_as_float(w[i]);
-            else { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-        }
+        const uint4* at = reinterpret_cast<const uint4*>(row + i0);
+        unpack_chunk<T>(__ldg(at), __ldg(at + 1), x);
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] = i0 + e >= 0 && i0 + e < V ? rb::to_f32(row[i0 + e]) : -INFINITY;
@@ -98,34 +105,39 @@ __device__ __forceinline__ void load_chunk(const T* row, int i0, int V, float* x
 }
 
 struct Shared {
-    Key lists[WARPS][32];
-    Sum sums[WARPS];
+    Key lists[MAX_BLOCKS][32];          // (as many as warps, or blocks of a cluster)
+    Sum sums[MAX_BLOCKS];
     Key best[32];             // this block's k most likely, sorted
+    Key leads[THREADS];       // largest elements of threads (by chunk), then candidates
     Sum sum;
+    unsigned int least[WARPS];
+    int n_leads, n_found;
 };
 
-// The 32 largest of all warps' sorted lists, sorted, in warp 0 (every thread calls this; `v`: the warp's list).
-__device__ __forceinline__ Key block_merge(Shared& sh, Key v) {
+// The 32 largest of the `lists` sorted lists (a power of two of them, at most 16; a warp brings its own in `v` where `mine`), sorted, in warp 0.  Every
+// thread calls this.
+__device__ __forceinline__ Key block_merge(Shared& sh, Key v, int lists = WARPS, bool mine = true) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    __syncthreads();
-    sh.lists[warp][lane] = v;
-#pragma unroll
-    for (int half = WARPS / 2; half > 0; half >>= 1) {
+    if (mine) {
+        __syncthreads();
+        sh.lists[warp][lane] = v;
+    }
+    for (int half = lists / 2; half > 0; half >>= 1) {
         __syncthreads();
         if (warp < half) {
-            v = warp_merge(v, sh.lists[warp + half][31 - lane]);
+            v = warp_merge(sh.lists[warp][lane], sh.lists[warp + half][31 - lane]);
             sh.lists[warp][lane] = v;
         }
     }
     return v;
 }
 
-// The warps' triples joined, by warp 0.
-__device__ __forceinline__ void sum_up(Shared& sh) {
+// `n` triples joined (at most 16), by warp 0.
+__device__ __forceinline__ void sum_up(Shared& sh, int n) {
     const int lane = threadIdx.x & 31;
-    Sum v = lane < WARPS ? sh.sums[lane] : Sum{NEG_BIG, 0.f, 0.f};
+    Sum v = lane < n ? sh.sums[lane] : Sum{NEG_BIG, 0.f, 0.f};
 #pragma unroll
-    for (int o = WARPS / 2; o > 0; o >>= 1) {
+    for (int o = MAX_BLOCKS / 2; o > 0; o >>= 1) {
         Sum other{__shfl_xor_sync(0xffffffffu, v.c, o), __shfl_xor_sync(0xffffffffu, v.s, o), __shfl_xor_sync(0xffffffffu, v.t, o)};
         v = join(v, other);
     }
@@ -133,7 +145,7 @@ __device__ __forceinline__ void sum_up(Shared& sh) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, Chunk<T>::BLOCKS_PER_SM)
 token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const int* __restrict__ ids, int m, float* __restrict__ logprobs,
                       float* __restrict__ entropy, float* __restrict__ top_logprobs, int* __restrict__ top_ids, int top, int blocks) {
     constexpr int E = Chunk<T>::E;
@@ -151,25 +163,80 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const i
     Sum mine{NEG_BIG, 0.f, 0.f};
     float best = -INFINITY;
     int best_chunk = lo + (int)threadIdx.x < hi ? lo + (int)threadIdx.x : -1;
-    for (int c = lo + threadIdx.x; c < hi; c += THREADS) {
-        float x[E];
-        load_chunk(row, c * E - before, V, x);
+    // A chunk's exponentials are added among themselves first: three hundred small terms, one by one, on top of a sum that already holds a large one
+    // would each be rounded at its size.
+    auto add_chunk = [&](const float* x) {
+        float s2[2] = {0.f, 0.f}, t2[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float d = max_nan(fmaf(x[e], LOG2E, -mine.c), -1000.f);       // (-inf: 2^-1000 is 0, and so is 0 times -1000)
+            const float p = rb::ex2(d);
+            s2[e & 1] += p;
+            t2[e & 1] = fmaf(d, p, t2[e & 1]);
+        }
+        mine.s += s2[0] + s2[1];
+        mine.t += t2[0] + t2[1];
+    };
+    auto largest = [&](const float* x) {
         float mx = x[0];
 #pragma unroll
         for (int e = 1; e < E; ++e) mx = fmaxf(mx, x[e]);
-        if (mx > best) { best = mx; best_chunk = c; }
+        return mx;
+    };
+    auto new_maximum = [&](float mx) {
         const float c_new = fmaxf(mine.c, mx * LOG2E);
-        const float f = rb::ex2(mine.c - c_new);
-        mine.t = mine.s > 0.f ? f * fmaf(mine.c - c_new, mine.s, mine.t) : f * mine.s;
-        mine.s *= f;
-        mine.c = c_new;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float d = max_nan(fmaf(x[e], LOG2E, -c_new), -1000.f);       // (-inf: 2^-1000 is 0, and so is 0 times -1000)
-            const float p = rb::ex2(d);
-            mine.s += p;
-            mine.t = fmaf(d, p, mine.t);
+        if (c_new > mine.c) {
+            const float f = rb::ex2(mine.c - c_new);
+            mine.t = mine.s > 0.f ? f * fmaf(mine.c - c_new, mine.s, mine.t) : f * mine.s;
+            mine.s *= f;
+            mine.c = c_new;
         }
+    };
+    // whole chunks, UNROLL of them at a time; the row's first and last chunk, which it may share with its neighbours, one by one
+    const int inner_lo = max(lo, before > 0 ? 1 : 0), inner_hi = min(hi, (int)(((long long)V + before) / E));
+    int c = lo + threadIdx.x;
+    if (c < hi && c < inner_lo) {
+        float x[E];
+        load_chunk(row, c * E - before, V, x);
+        best = largest(x);
+        new_maximum(best);
+        add_chunk(x);
+        c += THREADS;
+    }
+    for (; c < inner_hi; c += UNROLL * THREADS) {
+        uint4 raw[UNROLL][2];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const uint4* at = reinterpret_cast<const uint4*>(row + ((long long)min(c + u * THREADS, inner_hi - 1) * E - before));
+            raw[u][0] = __ldg(at);
+            raw[u][1] = __ldg(at + 1);
+        }
+        float mx[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            float x[E];
+            unpack_chunk<T>(raw[u][0], raw[u][1], x);
+            mx[u] = largest(x);
+            if (c + u * THREADS < inner_hi && mx[u] > best) { best = mx[u]; best_chunk = c + u * THREADS; }
+        }
+        float all = mx[0];
+#pragma unroll
+        for (int u = 1; u < UNROLL; ++u) all = fmaxf(all, mx[u]);
+        new_maximum(all);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            float x[E];
+            unpack_chunk<T>(raw[u][0], raw[u][1], x);
+            if (c + u * THREADS < inner_hi) add_chunk(x);
+        }
+    }
+    if (inner_hi < hi && hi - 1 >= inner_lo && (hi - 1 - lo) % THREADS == (int)threadIdx.x) {
+        float x[E];
+        load_chunk(row, (hi - 1) * E - before, V, x);
+        const float mx = largest(x);
+        if (mx > best) { best = mx; best_chunk = hi - 1; }
+        new_maximum(mx);
+        add_chunk(x);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -178,60 +245,127 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const i
     }
     if (lane == 0) sh.sums[warp] = mine;
     __syncthreads();
-    if (warp == 0) sum_up(sh);
+    if (warp == 0) sum_up(sh, WARPS);
     if (top > 0) {
-        // the threads whose largest elements lead (by value, then chunk: chunks of different threads differ)
-        Key v = block_merge(sh, warp_sort(best_chunk >= 0 ? key_of(best, best_chunk) : 0ull));
-        if (warp == 0) sh.best[lane] = v;
+        // 1. A bound that at least `top` threads' largest elements reach: the least of the warps' j-th largest, j = top / WARPS rounded up.  The
+        //    threads that reach it (some fifty for a top of 20) are put in a list.
+        const unsigned int mine_top = best_chunk >= 0 ? (unsigned int)(key_of(best, best_chunk) >> 32) : 0u;
+        unsigned int left = mine_top, jth = 0u;
+        for (int j = 0; j < top; j += WARPS) {
+            jth = __reduce_max_sync(0xffffffffu, left);
+            if (lane == __ffs(__ballot_sync(0xffffffffu, left == jth)) - 1) left = 0u;
+        }
+        if (threadIdx.x == 0) sh.n_leads = sh.n_found = 0;
+        if (lane == 0) sh.least[warp] = jth;
+        if (threadIdx.x < 32) sh.best[threadIdx.x] = 0ull;
         __syncthreads();
-        const Key last = sh.best[top - 1];
-        const float least = last ? key_value(last) : -INFINITY;
-        Key found = 0ull;
-        for (int j = warp; j < top; j += WARPS) {
-            const Key lead = sh.best[j];
-            if (!lead) break;
-            const int c0 = lo + (key_index(lead) - lo) % THREADS;
-            for (int cb = c0; cb < hi; cb += 32 * THREADS) {
-                const int c = cb + lane * THREADS, i0 = c * E - before;
-                float x[E];
-                if (c < hi) load_chunk(row, i0, V, x);
+        unsigned int bound = sh.least[0];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) bound = min(bound, sh.least[w]);
+        if (best_chunk >= 0 && mine_top >= bound) sh.leads[atomicAdd(&sh.n_leads, 1)] = key_of(best, best_chunk);
+        __syncthreads();
+        // 2. The `top` first of them, by how many are ahead of each (by value, then chunk: chunks of different threads differ).
+        const int n_leads = sh.n_leads;
+        if ((int)threadIdx.x < n_leads) {
+            const Key k = sh.leads[threadIdx.x];
+            int ahead = 0;
+            for (int i = 0; i < n_leads; ++i) ahead += sh.leads[i] > k;
+            if (ahead < top) sh.best[ahead] = k;
+        }
+        __syncthreads();
+        // 3. Their elements again, a chunk a thread, all chunks of all of them at once; what reaches the last one's value is a candidate.
+        const int n_top = min(top, n_leads), share = (hi - lo + THREADS - 1) / THREADS;
+        const float least = n_top == top ? key_value(sh.best[top - 1]) : -INFINITY;
+        for (int i0 = threadIdx.x; i0 < n_top * share; i0 += 2 * THREADS) {
+            float x[2][E];
+            int c2[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int i = i0 + u * THREADS;
+                c2[u] = i < n_top * share ? lo + (key_index(sh.best[i / share]) - lo) % THREADS + i % share * THREADS : hi;
+                if (c2[u] < hi) load_chunk(row, c2[u] * E - before, V, x[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (c2[u] >= hi) continue;
+                const int first = c2[u] * E - before;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    // (what is not ahead of the k-th found so far is not sorted in: rows of many equal values end quickly)
-                    const bool may = c < hi && i0 + e >= 0 && i0 + e < V && x[e] >= least;
-                    if (!__any_sync(0xffffffffu, may)) continue;
-                    Key key = may ? key_of(x[e], i0 + e) : 0ull;
-                    if (!__any_sync(0xffffffffu, key > __shfl_sync(0xffffffffu, found, top - 1))) continue;
-                    key = warp_sort(key);
-                    found = warp_merge(found, __shfl_sync(0xffffffffu, key, 31 - lane));
+                    if (x[u][e] >= least && first + e >= 0 && first + e < V) {
+                        const int at = atomicAdd(&sh.n_found, 1);
+                        if (at < THREADS) sh.leads[at] = key_of(x[u][e], first + e);
+                    }
                 }
             }
         }
-        v = block_merge(sh, found);
-        if (warp == 0) sh.best[lane] = v;
+        __syncthreads();
+        const int n_found = sh.n_found;
+        if (n_found <= THREADS) {
+            // 4. The first `top` candidates, counted the same way.
+            const Key k = (int)threadIdx.x < n_found ? sh.leads[threadIdx.x] : 0ull;
+            int ahead = 0;
+            for (int i = 0; i < n_found; ++i) ahead += sh.leads[i] > k;
+            if (threadIdx.x < 32) sh.best[threadIdx.x] = 0ull;
+            __syncthreads();
+            if (k && ahead < 32) sh.best[ahead] = k;
+        } else {
+            // Too many equal values: the same elements sorted in by warps.  (What is not ahead of the top-th found so far is not sorted in: rows
+            // of many equal values end quickly.)
+            Key found = 0ull;
+            for (int j = warp; j < n_top; j += WARPS) {
+                const int c0 = lo + (key_index(sh.best[j]) - lo) % THREADS;
+                for (int cb = c0; cb < hi; cb += 32 * THREADS) {
+                    const int c1 = cb + lane * THREADS, first = c1 * E - before;
+                    float x[E];
+                    if (c1 < hi) load_chunk(row, first, V, x);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const bool may = c1 < hi && first + e >= 0 && first + e < V && x[e] >= least;
+                        if (!__any_sync(0xffffffffu, may)) continue;
+                        Key key = may ? key_of(x[e], first + e) : 0ull;
+                        if (!__any_sync(0xffffffffu, key > __shfl_sync(0xffffffffu, found, top - 1))) continue;
+                        key = warp_sort(key);
+                        found = warp_merge(found, __shfl_sync(0xffffffffu, key, 31 - lane));
+                    }
+                }
+            }
+            found = block_merge(sh, found);
+            if (warp == 0) sh.best[lane] = found;
+        }
     }
     __syncthreads();
     if (blocks > 1) {
-        // the first block of the cluster reads what the others found, a warp a block
+        // the first block of the cluster reads what the others found, a warp up to two of them
         sm100::cluster_arrive();
         sm100::cluster_wait();
         if (part == 0) {
-            Sum v{NEG_BIG, 0.f, 0.f};
-            Key k = 0ull;
-            if (warp < blocks) {
-                const uint32_t at = sm100::map_to_cta(sm100::smem_u32(&sh.sum), warp);
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v.c) : "r"(at));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v.s) : "r"(at + 4));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v.t) : "r"(at + 8));
+            Sum v[2];
+            Key k[2] = {0ull, 0ull};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int p = warp + i * WARPS;
+                if (p >= blocks) continue;
+                const uint32_t at = sm100::map_to_cta(sm100::smem_u32(&sh.sum), p);
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[i].c) : "r"(at));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[i].s) : "r"(at + 4));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[i].t) : "r"(at + 8));
                 if (top > 0)
-                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(sm100::map_to_cta(sm100::smem_u32(&sh.best[lane]), warp)));
+                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k[i]) : "r"(sm100::map_to_cta(sm100::smem_u32(&sh.best[lane]), p)));
             }
-            if (lane == 0) sh.sums[warp] = v;
-            if (top > 0) k = block_merge(sh, k);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int p = warp + i * WARPS;
+                if (p >= blocks) continue;
+                if (lane == 0) sh.sums[p] = v[i];
+                sh.lists[p][lane] = k[i];
+            }
+            Key all_best = 0ull;
+            if (top > 0) all_best = block_merge(sh, 0ull, blocks, false);
             __syncthreads();
             if (warp == 0) {
-                sum_up(sh);
-                if (top > 0) sh.best[lane] = k;
+                sum_up(sh, blocks);
+                if (top > 0) sh.best[lane] = all_best;
             }
             __syncthreads();
         }

@@ -28,6 +28,7 @@ tree_accept_kernel(const int* __restrict__ tokens, const int* __restrict__ paren
     __shared__ int first[MAX_NODES], way[MAX_NODES];
     __shared__ unsigned int like_bits[WORDS];
     __shared__ int count;
+    __shared__ int2 pages[MAX_NODES];
     const int b = blockIdx.y, tid = threadIdx.x;
     const int slot = seq_slot ? seq_slot[b] : 0, q0 = cu_q[b];
     const int n = min(min(cu_q[b + 1] - q0, words * 32), path_ld);
@@ -74,34 +75,31 @@ tree_accept_kernel(const int* __restrict__ tokens, const int* __restrict__ paren
     if (!k) return;
     const int len = kv_len[b], ctx = len - (cu_q[b + 1] - q0);
     if (ctx < 0 || len > max_pages * RB_PAGE) return;
+    // where the path's nodes lie and belong, as rows of a layer's first head (-1: nothing to move; a node that is where it belongs stays)
+    if (tid < n_path) {
+        const int* table = block_table + (size_t)slot * max_pages;
+        const int node = way[tid], src = ctx + node, dst = ctx + tid;
+        int from = -1, to = -1;
+        if (node > tid) { from = table[src / RB_PAGE]; to = table[dst / RB_PAGE]; }
+        first[tid] = from >= 0 && to >= 0 ? src % RB_PAGE : -1;
+        pages[tid] = make_int2(from, to);
+    }
+    __syncthreads();
     // this thread's 16 bytes: unit (keys or values, layer, head) and place inside the head's row
-    const long long at = (long long)blockIdx.x * THREADS + tid;
-    const int unit = (int)(at / vecs), col = (int)(at % vecs);
-    if (unit >= 2 * units) return;
-    Vec* cache = unit < units ? k : v;
-    const int lh = unit < units ? unit : unit - units, layer = lh / nkv, head = lh % nkv;
-    const int* table = block_table + (size_t)slot * max_pages;
-    auto row = [&](int place) -> Vec* {
-        const int page = table[place / RB_PAGE];
-        if (page < 0) return nullptr;
-        return cache + ((((size_t)layer * n_pages + page) * nkv + head) * RB_PAGE + place % RB_PAGE) * vecs + col;
-    };
-    for (int d0 = 0; d0 < n_path; d0 += BATCH) {
-        Vec x[BATCH];
-        Vec* to[BATCH];
+    for (long long at = (long long)blockIdx.x * THREADS + tid; at < 2ll * units * vecs; at += (long long)gridDim.x * THREADS) {
+        const int unit = (int)(at / vecs), col = (int)(at % vecs);
+        const int lh = unit < units ? unit : unit - units, layer = lh / nkv, head = lh % nkv;
+        Vec* base = (unit < units ? k : v) + (((size_t)layer * n_pages) * nkv + head) * RB_PAGE * vecs + col;
+        const size_t page_step = (size_t)nkv * RB_PAGE * vecs;
+        for (int d0 = 0; d0 < n_path; d0 += BATCH) {
+            Vec x[BATCH];
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int d = d0 + i, node = d < n_path ? way[d] : -1;
-            to[i] = nullptr;
-            if (node > d) {                          // (a node that is where it belongs stays)
-                const Vec* from = row(ctx + node);
-                to[i] = from ? row(ctx + d) : nullptr;
-                if (to[i]) x[i] = *from;
-            }
+            for (int i = 0; i < BATCH; ++i)
+                if (d0 + i < n_path && first[d0 + i] >= 0) x[i] = base[pages[d0 + i].x * page_step + first[d0 + i] * vecs];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i)
+                if (d0 + i < n_path && first[d0 + i] >= 0) base[pages[d0 + i].y * page_step + (ctx + d0 + i) % RB_PAGE * vecs] = x[i];
         }
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i)
-            if (to[i]) *to[i] = x[i];
     }
 }
 
@@ -112,8 +110,10 @@ int launch_accept(const int* tokens, const int* parents, const int* visible, int
     const int vecs = row_bytes / (int)sizeof(Vec);
     const long long threads = k ? 2ll * layers * nkv * vecs : 1;
     const long long blocks = (threads + THREADS - 1) / THREADS;
-    if (blocks > 0x7fffffffll) return RB_ERR_BAD_SIZE;
-    RB_LAUNCH((tree_accept_kernel<Vec>), dim3((unsigned)blocks, n_seqs), dim3(THREADS), 0, stream, tokens, parents, visible, words, sampled, cu_q,
+    // about one wave of blocks over all sequences: each finds the path once, whatever it moves
+    const long long wave = (5 * 148 + n_seqs - 1) / n_seqs;
+    const unsigned x_blocks = (unsigned)(blocks < wave ? blocks : wave);
+    RB_LAUNCH((tree_accept_kernel<Vec>), dim3(x_blocks, n_seqs), dim3(THREADS), 0, stream, tokens, parents, visible, words, sampled, cu_q,
               path, path_ld, counts, next_token, seq_slot, kv_len, block_table, max_pages, (Vec*)k, (Vec*)v, layers * nkv, nkv, n_pages, vecs);
     return RB_OK;
 }

@@ -978,13 +978,13 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     longest = max_pages if max_kv_len is None else max(1, min(max_pages, (int(max_kv_len) + PAGE - 1) // PAGE))
     device = q.device
     group = nq // nkv
-    slots = _decode_slots(device)                      # three blocks of the plain kernel a multiprocessor
+    slots = _decode_slots(device) // 3 * 2             # two blocks a multiprocessor
     rows_tile = _TREE_ROWS
     pointers = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
     if dtype is torch.bfloat16 and hd in (64, 128, 256) and group <= 128 and not \
             ((pointers[0] | pointers[1] | pointers[2] | pointers[3]) & 15 or (q_stride | o_stride) & 7):
         rows_tile = 128 // group * group               # the tensor-core kernel: whole nodes in 128 rows
-        slots = slots // 3 * (2 if hd <= 128 else 1)
+        slots = slots if hd <= 128 else slots // 2
     units = n_seqs * -(-max_nodes * group // rows_tile)
     shares = tree_shares(longest * units, min(rows_tile, max_nodes * group), nkv, slots)
     work = None
@@ -1045,10 +1045,13 @@ LOGPROBS_MAX_TOP = 32
 
 
 def logprob_blocks(rows: int, vocab: int, device=0) -> int:
-    """Blocks a row of token_logprobs: as many as keep the device full once, a power of two up to 16, none with less than 2,048 logits."""
-    slots = 2 * _decode_slots(device) // 3
+    """Blocks a row of token_logprobs: a power of two that about fills the device once, none with less than 2,048 logits; up to eight, which any
+    cluster may have, and sixteen for a few rows only (151,936 logits, 20 alternatives: one row 7.6 us with sixteen, 8.1 with eight, 32 rows 18 and
+    13; 148 rows 31 with four, which would just fit, 24 with two)."""
+    slots = 7 * _decode_slots(device) // 6             # seven eighths of four blocks a multiprocessor
+    most = 16 if rows <= 8 else 8
     blocks = 1
-    while blocks < 16 and rows * blocks * 2 <= slots and vocab // (blocks * 2) >= 2048:
+    while blocks < most and rows * blocks * 2 <= slots and vocab // (blocks * 2) >= 2048:
         blocks *= 2
     return blocks
 
