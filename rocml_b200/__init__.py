@@ -12,14 +12,14 @@ from .errors import (
     CacheError, CacheFull, ConfigError, ContextOverflow, ExtensionMissing, KernelError,
     MemoryBudget, ModelFileMissing, RocmlError, SafetensorsError, UnknownModel, UnsupportedArchitecture, WeightsError,
 )
-from .engine import Engine, Model, StepEntry
+from .engine import Engine, Model, PromptLookup, StepEntry, TreeEntry
 from .engine.generate import Completion, GenerateStats, Request, generate
-from .sampling import SamplingParams
+from .sampling import SamplingParams, TokenScore
 
 __version__ = "0.1.0"
 
 __all__ = [
-    "config", "parts", "Engine", "Model", "StepEntry", "Completion", "GenerateStats", "Request",
+    "config", "parts", "Engine", "Model", "StepEntry", "TreeEntry", "PromptLookup", "TokenScore", "Completion", "GenerateStats", "Request",
     "generate", "SamplingParams", "CacheError", "CacheFull", "ConfigError",
     "ContextOverflow", "ExtensionMissing", "KernelError", "MemoryBudget", "ModelFileMissing", "RocmlError",
     "SafetensorsError", "UnknownModel", "UnsupportedArchitecture", "WeightsError",

@@ -134,6 +134,16 @@ class KVGroup:
                 self._dirty.add(slot)
         self._released_upto[slot] = max(start, keep_from)
 
+    def trim(self, slot: int, length: int) -> None:
+        """Give back the pages that hold nothing but places >= length."""
+        row = self.table_host[slot]
+        for p in range(pages_for(length), self.max_pages_per_seq):
+            if row[p] < 0:
+                break
+            self.pool.free(int(row[p]))
+            row[p] = -1
+            self._dirty.add(slot)
+
     def release_all(self, slot: int) -> None:
         row = self.table_host[slot]
         for p in np.nonzero(row >= 0)[0]:
@@ -373,6 +383,12 @@ class SequenceCache:
         self.lengths[slot] += n_new
         for g in self.kv_groups:
             g.release_out_of_window(slot, self.lengths[slot])
+
+    def trim(self, slot: int) -> None:
+        """Give back the pages past the sequence's length (those of drafted tokens that it did not keep)."""
+        self._held(slot)
+        for g in self.kv_groups:
+            g.trim(slot, self.lengths[slot])
 
     def flush(self) -> None:
         for g in self.kv_groups:

@@ -86,7 +86,7 @@ tree_accept_kernel(const int* __restrict__ tokens, const int* __restrict__ paren
     }
     __syncthreads();
     // this thread's 16 bytes: unit (keys or values, layer, head) and place inside the head's row
-    for (long long at = (long long)blockIdx.x * THREADS + tid; at < 2ll * units * vecs; at += (long long)gridDim.x * THREADS) {
+    for (long long at = (long long)blockIdx.x * THREADS + tid; at < (v ? 2ll : 1ll) * units * vecs; at += (long long)gridDim.x * THREADS) {
         const int unit = (int)(at / vecs), col = (int)(at % vecs);
         const int lh = unit < units ? unit : unit - units, layer = lh / nkv, head = lh % nkv;
         Vec* base = (unit < units ? k : v) + (((size_t)layer * n_pages) * nkv + head) * RB_PAGE * vecs + col;
@@ -108,7 +108,7 @@ int launch_accept(const int* tokens, const int* parents, const int* visible, int
                   int* path, int path_ld, int* counts, int* next_token, const int* seq_slot, const int* kv_len, const int* block_table,
                   int max_pages, void* k, void* v, int layers, int nkv, long long n_pages, int row_bytes, cudaStream_t stream) {
     const int vecs = row_bytes / (int)sizeof(Vec);
-    const long long threads = k ? 2ll * layers * nkv * vecs : 1;
+    const long long threads = k ? (v ? 2ll : 1ll) * layers * nkv * vecs : 1;
     const long long blocks = (threads + THREADS - 1) / THREADS;
     // about one wave of blocks over all sequences: each finds the path once, whatever it moves
     const long long wave = (5 * 148 + n_seqs - 1) / n_seqs;
@@ -119,14 +119,14 @@ int launch_accept(const int* tokens, const int* parents, const int* visible, int
 }
 }  // namespace
 
-// k, v: [layers, n_pages, nkv, 64, row_bytes], or null (nothing is moved).
+// k, v: [layers, n_pages, nkv, 64, row_bytes]; v null: one tensor serves as both; both null: nothing is moved.
 extern "C" int rb_tree_accept(const int* tokens, const int* parents, const int* visible, int words, const int* sampled, const int* cu_q,
                               int n_seqs, int* path, int path_ld, int* counts, int* next_token, const int* seq_slot, const int* kv_len,
                               const int* block_table, int max_pages, void* k, void* v, int layers, int nkv, long long n_pages,
                               int row_bytes, int element_bytes, void* stream) {
     if (n_seqs <= 0) return RB_OK;
     if (words <= 0 || words > WORDS || path_ld <= 0 || path_ld > MAX_NODES || n_seqs > 65535) return RB_ERR_BAD_SIZE;
-    if ((k == nullptr) != (v == nullptr)) return RB_ERR_BAD_SIZE;
+    if ((v && !k) || (k && k == v)) return RB_ERR_BAD_SIZE;          // (one tensor for both is moved once)
     if (k && (!seq_slot || !kv_len || !block_table || layers <= 0 || nkv <= 0 || row_bytes <= 0 || max_pages <= 0)) return RB_ERR_BAD_SIZE;
     cudaStream_t st = (cudaStream_t)stream;
 #define RB_ACCEPT_ARGS tokens, parents, visible, words, sampled, cu_q, n_seqs, path, path_ld, counts, next_token, seq_slot, kv_len, block_table, \

@@ -26,14 +26,31 @@ class HostBatch:
     want_rows: List[int]
 
 
+@dataclass
+class TreeBatch:
+    """What parts see besides when the step's sequences bring trees of drafted tokens: node j of a sequence lies at place kv_len - n + j of
+    its pages (``StepBatch.positions``), its position in the text is another."""
+
+    positions: torch.Tensor       # int32 [T]: the context's length plus the node's depth
+    parents: torch.Tensor         # int32 [T]: within the tree, -1 for its first node
+    visible: torch.Tensor         # int32 [T, TREE_WORDS]: a bit for each of the node's ancestors and itself
+    max_nodes: int
+
+
+TREE_WORDS = 8                    # 32 nodes a word
+
+
 class BatchBuffers:
     """Fixed-capacity integer storage for a step's metadata: one device buffer, and a ring of
     pinned host buffers in front of it so that filling the next step's integers never
     overwrites a copy that is still in flight."""
 
-    def __init__(self, max_tokens: int, max_seqs: int, max_want: int, device, depth: int = 4):
+    def __init__(self, max_tokens: int, max_seqs: int, max_want: int, device, depth: int = 4, trees: bool = False):
         self.max_tokens, self.max_seqs, self.max_want = max_tokens, max_seqs, max_want
         sizes = [max_tokens, max_tokens, max_tokens, max_seqs, max_seqs + 1, max_seqs, max_want]
+        self.trees = trees
+        if trees:
+            sizes += [max_tokens, max_tokens, max_tokens * TREE_WORDS]
         self._offsets = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int64)
         total = int(self._offsets[-1])
         self.device = torch.device(device)
@@ -47,8 +64,9 @@ class BatchBuffers:
         return self.dev[int(self._offsets[i]):int(self._offsets[i + 1])]
 
     def fill(self, token_ids, positions, slot_of_token, cu_q, kv_len, want_rows, seq_slot,
-             pad_tokens: int, pad_seqs: int, pad_want: int) -> None:
-        """Write one step's integers (padded to the given counts) and copy them to the device."""
+             pad_tokens: int, pad_seqs: int, pad_want: int, tree=None) -> None:
+        """Write one step's integers (padded to the given counts) and copy them to the device.  ``tree``: (positions, parents, rows of
+        bits) of a step of trees."""
         T, B, W = len(token_ids), len(seq_slot), len(want_rows)
         if pad_tokens > self.max_tokens or pad_seqs > self.max_seqs or pad_want > self.max_want:
             raise ValueError("step does not fit the batch buffers")
@@ -69,6 +87,10 @@ class BatchBuffers:
         h(4)[:B + 1] = cu_q; h(4)[B + 1:pad_seqs + 1] = cu_q[-1]
         h(5)[:B] = kv_len; h(5)[B:pad_seqs] = 0
         h(6)[:W] = want_rows; h(6)[W:pad_want] = -1
+        if tree is not None:
+            h(7)[:T] = tree[0]; h(7)[T:pad_tokens] = 0
+            h(8)[:T] = tree[1]; h(8)[T:pad_tokens] = -1
+            h(9)[:T * TREE_WORDS] = tree[2].reshape(-1); h(9)[T * TREE_WORDS:pad_tokens * TREE_WORDS] = 0
         self.dev.copy_(host, non_blocking=True)
         if self._cuda:
             ev = torch.cuda.Event()
@@ -86,6 +108,9 @@ class BatchBuffers:
     cu_q = property(lambda s: s._d(4))
     kv_len = property(lambda s: s._d(5))
     want_rows = property(lambda s: s._d(6))
+
+    def tree(self, pad_tokens: int, max_nodes: int) -> TreeBatch:
+        return TreeBatch(self._d(7), self._d(8), self._d(9)[:pad_tokens * TREE_WORDS].view(pad_tokens, TREE_WORDS), max_nodes)
 
 
 @dataclass
@@ -109,6 +134,12 @@ class StepBatch:
     capturing: bool = False
     at_once: bool = True          # all layers as one kernel, where there is one, pay at these lengths (parts.decode_layers.pays)
     scratch: dict = field(default_factory=dict)
+    tree: Optional[TreeBatch] = None
+
+    @property
+    def angle_positions(self) -> torch.Tensor:
+        """Where the tokens stand in their texts: what a position encoding goes by (``positions`` says where their keys go)."""
+        return self.positions if self.tree is None else self.tree.positions
 
 
 def pack_entries(slots: Sequence[int], old_lens: Sequence[int], token_lists: Sequence[Sequence[int]],

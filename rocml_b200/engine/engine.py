@@ -171,6 +171,10 @@ class Engine:
         self._sampler = None
         self._device_tokens = None
         self._replayed = False     # the last piece's logits are a graph's
+        self._tree_graphs: "OrderedDict[Tuple[int, ...], dict]" = OrderedDict()
+        self._trees = None
+        self._scorer = None
+        self._last_buffers = None  # what the last graph was filled from
         self.graph_kernel_launches = 0  # kernels run by graph replays
 
     # After the weights are resident: does the cache fit what is left, with head room for a step's
@@ -384,16 +388,17 @@ class Engine:
 
     @staticmethod
     def _batch(buf: BatchBuffers, T, B, W, max_q, max_kv, is_decode, host, at_once=True, capturing=False) -> StepBatch:
+        # (a step of trees: the longest piece of a sequence is its largest tree)
         return StepBatch(
             n_tokens=T, n_seqs=B, n_want=W, max_q_len=max_q, max_kv_len=max_kv, is_decode=is_decode,
             token_ids=buf.token_ids, positions=buf.positions, slot_of_token=buf.slot_of_token,
             seq_slot=buf.seq_slot, cu_q=buf.cu_q, kv_len=buf.kv_len, want_rows=buf.want_rows, host=host,
-            capturing=capturing, at_once=at_once)
+            capturing=capturing, at_once=at_once, tree=buf.tree(T, max_q) if buf.trees else None)
 
-    def _run_graph(self, graphs, kept: int, key, packed, host, W, pads, at_once=True) -> Optional[torch.Tensor]:
+    def _run_graph(self, graphs, kept: int, key, packed, host, W, pads, at_once=True, tree=None) -> Optional[torch.Tensor]:
         """Replay the graph of ``key`` among ``graphs``, of which ``kept`` are kept, after capturing it if need be.  ``pads``: the
         tokens, sequences and wanted rows that it is sized for, the longest piece of a sequence, the longest sequence, whether it is
-        a step of single tokens."""
+        a step of single tokens.  ``tree``: what ``BatchBuffers.fill`` takes of a step of trees."""
         t_pad, b_pad, w_pad, max_q, ctx_pad, is_decode = pads
         B = len(host.seq_slots)
         g = graphs.get(key)
@@ -406,24 +411,26 @@ class Engine:
                 if old["graph"] is not None:
                     old["graph"].reset()
                 old.clear()
-            g = {"buffers": BatchBuffers(t_pad, b_pad, w_pad, self.device), "graph": None, "logits": None, "plain": False}
+            g = {"buffers": BatchBuffers(t_pad, b_pad, w_pad, self.device, trees=tree is not None), "graph": None, "logits": None, "plain": False}
             graphs[key] = g
         else:
             graphs.move_to_end(key)
         buf: BatchBuffers = g["buffers"]
-        buf.fill(*packed, host.seq_slots, pad_tokens=t_pad, pad_seqs=b_pad, pad_want=w_pad)
+        self._last_buffers = buf
+        buf.fill(*packed, host.seq_slots, pad_tokens=t_pad, pad_seqs=b_pad, pad_want=w_pad, tree=tree)
         if self._device_tokens is not None:
             buf.token_ids[:B].copy_(self._device_tokens, non_blocking=True)
         self.last_h2d_bytes = buf.h2d_bytes
         def batch(capturing=False):
             return self._batch(buf, t_pad, b_pad, w_pad, max_q, ctx_pad, is_decode, None if capturing else host, at_once, capturing)
-        if g["graph"] is None and not is_decode and not g["plain"]:
+        first_plainly = is_decode or tree is not None
+        if g["graph"] is None and not first_plainly and not g["plain"]:
             self._capture(g, batch(capturing=True))              # (a prompt of this size has run before)
         if g["graph"] is None:
-            # First use of a decode bucket: run it plainly (this also loads every kernel), then
+            # First use of a bucket of single tokens or trees: run it plainly (this also loads every kernel), then
             # capture the same launches for the next time.  Capturing executes nothing.
             out = self.model.forward(batch(), self.cache)
-            if is_decode and not g["plain"]:
+            if first_plainly and not g["plain"]:
                 torch.cuda.current_stream().synchronize()
                 self._capture(g, batch(capturing=True))
                 self.graphs_captured += g["graph"] is not None
@@ -444,7 +451,7 @@ class Engine:
         before = kernels.launch_count
         for _ in range(2):
             # (graphs share their memory, as no two run side by side; it goes with the last of them)
-            pool = next((x["graph"].pool() for t in (self._graphs, self._prompt_graphs) for x in t.values() if x["graph"] is not None), None)
+            pool = next((x["graph"].pool() for t in (self._graphs, self._prompt_graphs, self._tree_graphs) for x in t.values() if x["graph"] is not None), None)
             graph = torch.cuda.CUDAGraph()
             try:
                 with torch.cuda.stream(self._capture_stream):
@@ -466,6 +473,33 @@ class Engine:
             torch.cuda.empty_cache()
         g["plain"] = True
 
+    # ---- trees of drafted tokens, scoring ------------------------------------------------------------------
+    def _tree_steps(self):
+        if self._trees is None:
+            from .trees import TreeSteps
+            self._trees = TreeSteps(self)
+        return self._trees
+
+    def tree_logits(self, entries) -> torch.Tensor:
+        """Float32 logits [all nodes, vocab] of trees of drafted tokens (``TreeEntry``), every node behind its sequence's context and its
+        ancestors.  The sequences stay as long as they were.  The tensor may be reused by the next step."""
+        return self._tree_steps().logits(entries)
+
+    def verify(self, entries, params, rngs=None, histories=None) -> List[List[int]]:
+        """Run trees of drafted tokens and keep what the model itself would have drawn.  At every node a token is sampled (``params`` and ``rngs``, one
+        an entry; a sequence's nodes of one depth share the draw that the ordinary loop would have used there); a child with that token
+        is confirmed, and so on down.  Each sequence becomes longer by its first node and the confirmed ones; what comes back, an entry a
+        list, are the confirmed children's tokens and the token sampled after the last of them, which the sequence does not hold yet: the
+        tokens that as many ordinary steps would have sampled.  ``histories`` (an entry: prompt and tokens so far, the first node's
+        included) is read for repeat penalties only."""
+        return self._tree_steps().verify(entries, params, rngs, histories)
+
+    def score(self, sequences, top: int = 0):
+        """How likely every token of the given sequences is after the ones before it: a list of ``TokenScore`` a sequence (for its second token
+        on), with the ``top`` most likely tokens (at most 32) at its place."""
+        from .scoring import score
+        return score(self, sequences, top)
+
     # ---- generation: the engine as the loop's executor ------------------------------------------------------
     @property
     def max_seq_len(self) -> int:
@@ -477,11 +511,12 @@ class Engine:
     def capacity_slots(self) -> int:
         return self.cache.max_slots
 
-    def launch(self, slots, tokens, params, rngs, histories, feed_from=None):
+    def launch(self, slots, tokens, params, rngs, histories, feed_from=None, logprobs=None):
         """Enqueue a step of the sequences with their next tokens and the sampling of one token
         each, and return a handle at once.  With ``feed_from`` (the handle of the step before,
         over the same sequences in the same order) the next tokens are the ones that step
-        sampled, taken on the device: ``tokens`` is not read."""
+        sampled, taken on the device: ``tokens`` is not read.  ``logprobs`` (a number of alternatives): the sampled tokens are
+        scored too (``collect_scores``)."""
         device_tokens = None
         if feed_from is not None:
             if feed_from.n != len(slots):
@@ -502,10 +537,23 @@ class Engine:
                     logits = self.step([StepEntry(s, t, [len(t) - 1]) for s, t in zip(slots, tokens)],
                                        device_tokens=device_tokens)
                     with prof.scope(op="sampling"):
-                        return self._sampler.launch(logits, params, rngs, histories,
-                                                    status=kernels.status_word(self.device))
+                        return self._sample(logits, params, rngs, histories, logprobs)
         logits = self.step([StepEntry(s, t, [len(t) - 1]) for s, t in zip(slots, tokens)], device_tokens=device_tokens)
-        return self._sampler.launch(logits, params, rngs, histories, status=kernels.status_word(self.device))
+        return self._sample(logits, params, rngs, histories, logprobs)
+
+    def _sample(self, logits, params, rngs, histories, logprobs):
+        from .. import kernels
+        handle = self._sampler.launch(logits, params, rngs, histories, status=kernels.status_word(self.device))
+        if logprobs is not None:
+            if self._scorer is None:
+                from ..sampling import Scorer
+                self._scorer = Scorer(self.device, max_batch=max(self.cache.max_slots, 1))
+            handle.scores = self._scorer.launch(logits[:handle.n], handle.device_tokens[:handle.n], logprobs)
+        return handle
+
+    def collect_scores(self, handle):
+        """The ``TokenScore`` of every token of a launched step (``launch`` with ``logprobs``)."""
+        return self._scorer.collect(handle.scores)
 
     def collect(self, handle) -> List[int]:
         """Wait for a launched step and bring its token ids (nothing else) back to the host."""
@@ -517,15 +565,25 @@ class Engine:
         return self.collect(self.launch(slots, tokens, params, rngs, histories))
 
     def generate(self, prompts, max_new_tokens: int = 64, sampling=None, stop_tokens=None,
-                 ignore_eos: bool = False, max_batch: int = 64, on_token=None, stats=None, run_ahead: bool = True):
+                 ignore_eos: bool = False, max_batch: int = 64, on_token=None, stats=None, run_ahead: bool = True,
+                 logprobs: Optional[int] = None, drafter=None):
         """Generate for a list of prompts (token id lists).  Returns a list of Completion.
-        ``sampling`` is one SamplingParams for all or a list; stop tokens default to the model's."""
+        ``sampling`` is one SamplingParams for all or a list; stop tokens default to the model's.  ``logprobs``: every token comes with
+        its log probability and so many alternatives (0 to 32).  ``drafter``: drafts of the tokens that may follow, verified several at a
+        time (``engine.drafting``); the tokens are the same without it."""
         from ..sampling import SamplingParams
         from .generate import Request, generate
         if sampling is None:
             sampling = SamplingParams()
+        if logprobs is not None:
+            from ..sampling.scorer import check_top
+            logprobs = check_top(logprobs, self.model.vocab)
         per = sampling if isinstance(sampling, (list, tuple)) else [sampling] * len(prompts)
-        reqs = [Request(list(p), max_new_tokens, sp, stop_tokens, ignore_eos) for p, sp in zip(prompts, per)]
+        reqs = [Request(list(p), max_new_tokens, sp, stop_tokens, ignore_eos, logprobs) for p, sp in zip(prompts, per)]
+        if drafter is not None:
+            from .drafting import generate_drafted
+            return generate_drafted(self, reqs, drafter, default_stop=self.model.spec.stop_tokens, max_batch=max_batch,
+                                    on_token=on_token, stats=stats)
         return generate(self, reqs, default_stop=self.model.spec.stop_tokens, max_batch=max_batch,
                         on_token=on_token, stats=stats, run_ahead=run_ahead)
 

@@ -37,6 +37,7 @@ class Request:
     sampling: SamplingParams = SamplingParams()
     stop_tokens: Optional[Iterable[int]] = None   # None: the model's own stop tokens
     ignore_eos: bool = False                      # keep going through stop tokens (benchmarks)
+    logprobs: Optional[int] = None                # score every token, with so many alternatives
 
 
 @dataclass
@@ -44,6 +45,7 @@ class Completion:
     tokens: List[int]
     finish_reason: str        # "stop", "length" (token budget) or "context" (no room left)
     prompt_tokens: int
+    logprobs: Optional[list] = None   # a TokenScore for every token, when the request asked
 
 
 @dataclass
@@ -83,6 +85,7 @@ class Executor(Protocol):
     # def launch(self, slots, tokens, params, rngs, histories, feed_from=None) -> handle
     #     the same, enqueued only; with feed_from (the handle of the step before, same sequences,
     #     same order) the next tokens are that step's samples and ``tokens`` is not read
+    #     (with logprobs=k, only given when a request asks: ``collect_scores(handle)`` then gives a TokenScore a token)
     # def collect(self, handle) -> List[int]
 
 
@@ -158,10 +161,13 @@ def generate(executor: Executor, requests: Sequence[Request], default_stop: Iter
             raise RocmlError(f"request {i} has an empty prompt")
         if len(r.prompt) > limit:
             raise RocmlError(f"request {i}: prompt of {len(r.prompt)} tokens exceeds the context of {limit}")
+        if r.logprobs is not None and not hasattr(executor, "collect_scores"):
+            raise RocmlError(f"request {i}: this executor does not score tokens")
         needs.append(min(len(r.prompt) + max(r.max_new_tokens, 0), limit))
     results: List[Optional[Completion]] = [None] * len(requests)
+    scored = any(r.logprobs is not None for r in requests)
     pipelined = run_ahead and hasattr(executor, "launch") and hasattr(executor, "collect")
-    ex = executor if pipelined else _Sync(executor)
+    ex = executor if pipelined or scored else _Sync(executor)
     for batch in plan_batches(needs, max_batch, executor.capacity_tokens(), executor.capacity_slots()):
         stats.batches += 1
         live = []
@@ -171,16 +177,19 @@ def generate(executor: Executor, requests: Sequence[Request], default_stop: Iter
                 results[i] = Completion([], "length", len(r.prompt))
                 continue
             stops = default_stop if r.stop_tokens is None else set(r.stop_tokens)
-            live.append({"i": i, "req": r, "slot": executor.new_sequence(), "out": [], "done": False,
+            live.append({"i": i, "req": r, "slot": executor.new_sequence(), "out": [], "done": False, "scores": [],
                          "history": list(r.prompt), "stops": stops,
                          "rng": XorShift64Star(r.sampling.seed + j), "next": list(r.prompt)})
         if not live:
             continue
 
+        tops = [s["req"].logprobs for s in live if s["req"].logprobs is not None]
+        asked = {"logprobs": max(tops)} if tops else {}
+
         def launch(seqs, feed_from=None):
             return ex.launch([s["slot"] for s in seqs], [s["next"] for s in seqs],
                              [s["req"].sampling for s in seqs], [s["rng"] for s in seqs],
-                             [s["history"] for s in seqs], feed_from=feed_from)
+                             [s["history"] for s in seqs], feed_from=feed_from, **asked)
 
         t_batch = time.perf_counter()
         flying, handle = live, launch(live)      # the step whose tokens are read next
@@ -191,9 +200,10 @@ def generate(executor: Executor, requests: Sequence[Request], default_stop: Iter
             if pipelined and all(_goes_on_for_sure(s, limit) for s in flying):
                 ahead = launch(flying, feed_from=handle)
             tokens = ex.collect(handle)
+            scores = ex.collect_scores(handle) if asked else [None] * len(tokens)
             still = []
             n_read = 0
-            for s, tok in zip(flying, tokens):
+            for s, tok, score in zip(flying, tokens, scores):
                 if s["done"]:
                     continue                      # it ended while this step was already on its way
                 n_read += 1
@@ -204,6 +214,9 @@ def generate(executor: Executor, requests: Sequence[Request], default_stop: Iter
                 if emit:
                     s["out"].append(tok)
                     s["history"].append(tok)
+                    if r.logprobs is not None:
+                        score.top = score.top[:r.logprobs]
+                        s["scores"].append(score)
                     if on_token is not None and on_token(s["i"], tok) and reason is None:
                         reason = "stop"       # the callback sees every emitted token; its answer ends a sequence that would go on
                 if reason is None:
@@ -212,7 +225,7 @@ def generate(executor: Executor, requests: Sequence[Request], default_stop: Iter
                 else:
                     s["done"] = True
                     executor.release(s["slot"])
-                    results[s["i"]] = Completion(s["out"], reason, len(r.prompt))
+                    results[s["i"]] = Completion(s["out"], reason, len(r.prompt), s["scores"] if r.logprobs is not None else None)
             if ahead is not None and not still:
                 ex.collect(ahead)                 # everyone ended: nothing of that step is kept
                 ahead = None

@@ -131,6 +131,11 @@ class Model:
 
     # ---- facts ----------------------------------------------------------------------------------
     @property
+    def takes_trees(self) -> bool:
+        """Whether a step may bring trees of drafted tokens: nothing is kept but keys and values, and every mixer says that it can."""
+        return all(isinstance(r, KVRequirement) for r in self.cache_requirements()) and all(getattr(getattr(b, "mixer", None), "takes_trees", False) for b in self.blocks)
+
+    @property
     def graph_safe(self) -> bool:
         return all(b.graph_safe for b in self.blocks) and self.final_norm.graph_safe and \
             (self.embedding_norm is None or self.embedding_norm.graph_safe)
@@ -197,7 +202,7 @@ class Model:
             if self.input_position is None and self.spec.embedding_scale == 1.0 and (x0 is None or rows is not resid):
                 kernels.embedding(batch.token_ids, self.embed, rows, self.status)
             else:
-                kernels.embedding_pos(batch.token_ids, self.embed, rows, self.spec.embedding_scale, batch.positions,
+                kernels.embedding_pos(batch.token_ids, self.embed, rows, self.spec.embedding_scale, batch.angle_positions,
                                       self.input_position.inv_freq if self.input_position is not None else None,
                                       copy=x0 if rows is resid else None, status=self.status,
                                       pos_table=getattr(self.input_position, "table", None))

@@ -1007,7 +1007,8 @@ def tree_accept(token_ids: torch.Tensor, parents: torch.Tensor, visible: torch.T
     rows of ancestor bits ``visible``) the tokens that were sampled at the nodes confirm.  Node 0 always is; a node below it when its parent is
     and the parent's sampled token is its own (of several such children the first).  path int32 [n_seqs, >= the largest tree] receives the confirmed
     nodes from node 0 down, -1 behind them, counts [n_seqs] how many they are, next_token [n_seqs] the token sampled at the last one.
-    With ``k`` and ``v`` [layers, pages, nkv, 64, hd] (and seq_slot, kv_len, block_table as for ``attention_tree``) their keys and values are moved
+    With ``k`` and ``v`` [layers, pages, nkv, 64, hd] (``v`` None: one tensor serves as both; and seq_slot, kv_len, block_table as for
+    ``attention_tree``) their keys and values are moved
     to the places kv_len - n + 0, 1, 2, ... in every layer.  Rows of slots below 0 stay as they are.  Parents come before their
     children."""
     if path.dim() != 2 or path.shape[0] < n_seqs or visible.dim() != 2:
@@ -1019,13 +1020,15 @@ def tree_accept(token_ids: torch.Tensor, parents: torch.Tensor, visible: torch.T
         raise KernelError(f"tree_accept: path holds at most {TREE_MAX_NODES} nodes a sequence")
     layers = nkv = row_bytes = esz = 0
     n_pages = max_pages = 0
-    if (k is None) != (v is None):
-        raise KernelError("tree_accept: keys and values come together")
+    if v is not None and (k is None or k.dtype is not v.dtype or k.shape != v.shape or not v.is_contiguous()):
+        raise KernelError("tree_accept: values come with keys like them")
     if k is not None:
         if seq_slot is None or kv_len is None or block_table is None or seq_slot.numel() < n_seqs or kv_len.numel() < n_seqs:
             raise KernelError("tree_accept: moving keys and values needs seq_slot, kv_len and block_table")
-        if k.dim() != 5 or k.shape[3] != PAGE or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or not v.is_contiguous():
+        if k.dim() != 5 or k.shape[3] != PAGE or not k.is_contiguous() or block_table.dim() != 2:
             raise KernelError("tree_accept: k and v must be contiguous [layers, pages, nkv, 64, hd]")
+        if v is not None and v.data_ptr() == k.data_ptr():
+            v = None                       # one tensor serves as both: it is moved once
         layers, n_pages, nkv = k.shape[0], k.shape[1], k.shape[2]
         esz = k.element_size()
         row_bytes, max_pages = k.shape[4] * esz, block_table.shape[1]

@@ -182,6 +182,12 @@ class Attention(Mixer):
             return BundleRequirement.of(req, conv=StateRequirement((self.conv_taps - 1, self.conv_channels), torch.float32))
         return req
 
+    @property
+    def takes_trees(self) -> bool:
+        """Masks by blocks of positions, mixed heads and what is kept beside keys and values have no form for trees; a temperature goes
+        by the place of a key in the cache, which is not a drafted token's position."""
+        return not (self.chunk or self.talking_heads or self.conv_taps or self.q_temp)
+
     def _span(self) -> int:
         """The mask as the kernels take it: 0 every earlier key, n the last n keys, -n blocks of n positions."""
         if self.window:
@@ -531,8 +537,17 @@ def paged_attention(q, out, batch, k_cache, v_cache, block_table, nq, nkv, hd, s
     such pages calls this (keys and values may be the same tensor).  ``gate``: nq * hd columns of the step's projection
     rows ([T, ..] or partial sums [S, T, ..]); a kernel that takes them multiplies its result by their sigmoid.
     Returns whether that was done: if not, the result is as without ``gate`` and the caller gates it.
+    A step of trees of drafted tokens (``batch.tree``): every node sees its sequence's context and its ancestors.
     ``cross`` (n > 1, the cache's own number of key/value heads): every query head's weights are applied to the values of
     every stored head; nkv = n * n then counts (key head, value head) pairs and nq = n * query heads the results."""
+    if batch.tree is not None:
+        if cross > 1 or window < 0:
+            raise ConfigError("attention: mixed heads and masks by blocks of positions do not take trees of drafted tokens")
+        t = batch.tree
+        kernels.attention_tree(q, out, k_cache, v_cache, block_table, batch.seq_slot, batch.cu_q, batch.kv_len, t.visible, batch.n_seqs,
+                               t.max_nodes, nq, nkv, hd, scale, max_kv_len=batch.max_kv_len, positions=t.positions, window=window, keep=keep,
+                               sink=sink, softcap=softcap)
+        return False
     if batch.is_decode:
         chunk = DECODE_CHUNK
         T = batch.n_tokens

@@ -202,7 +202,10 @@ class Mixer(Part):
     """forward(xn [T, H], batch, view) -> delta [S, T, H] float32 to be added to the residual.
 
     ``cache_requirement()`` says what the cache must keep for this layer: a KVRequirement,
-    a StateRequirement or None."""
+    a StateRequirement or None.  ``takes_trees``: forward() heeds ``batch.tree``, a step whose sequences bring trees of
+    drafted tokens instead of the tokens that follow."""
+
+    takes_trees = False
 
     def cache_requirement(self):
         return None

@@ -99,6 +99,8 @@ class LatentAttention(Mixer):
         self.fold: Optional[torch.Tensor] = None       # [heads, kv_rank, head_dim]: Wuk_h^T
         self.unfold: Optional[torch.Tensor] = None     # [heads, v_head_dim, kv_rank]: Wuv_h
 
+    takes_trees = True       # (a latent is cached where its token's place says, its rotated part turned by its position)
+
     def cache_requirement(self):
         return KVRequirement(1, self.dp, self.window, shared_values=True)
 

@@ -38,6 +38,7 @@ class PendingSample:
     host_tokens: torch.Tensor
     host_status: Optional[torch.Tensor]
     event: "torch.cuda.Event"
+    scores: object = None         # a PendingScores, when the tokens are scored too
 
 
 class Sampler:

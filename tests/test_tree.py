@@ -175,7 +175,7 @@ def _accept(**change):
     ({"counts": torch.zeros(1, dtype=torch.int32)}, "for every sequence"),
     ({"path": torch.zeros((2, 300), dtype=torch.int32)}, "at most 256"),
     ({"path": torch.zeros((1, 4), dtype=torch.int32)}, "n_seqs"),
-    ({"k": torch.zeros((1, 2, 1, 64, 16))}, "come together"),
+    ({"v": torch.zeros((1, 2, 1, 64, 16))}, "come with keys"),
     ({"k": torch.zeros((1, 2, 1, 64, 16)), "v": torch.zeros((1, 2, 1, 64, 16))}, "needs seq_slot"),
 ])
 def test_tree_accept_refuses(change, says):
