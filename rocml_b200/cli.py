@@ -1,4 +1,4 @@
-"""Command line: ``python -m rocml_b200 {generate,bench,models}``.
+"""Command line: ``python -m rocml_b200 {generate,score,bench,models}``.
 
 The commands, option names and meanings follow the reference's ``rocml-cli``
 (rocml-cli/src/main.rs:26-38): ``--model <name-or-path>`` (common.rs:42-43), ``-n/--max-tokens``
@@ -11,7 +11,8 @@ table against the device's limits after the run and ``--profile-json`` writes it
 they lie outside this library: prompts are token ids (``--prompt-ids`` / ``--prompt-file`` /
 ``--prompt-len``; there is no tokenizer here), and ``--random`` generates seeded random weights for
 a named size instead of downloading a checkpoint.  ``--dtype`` takes the place of ``--kv-cache``:
-it selects the whole path (bfloat16 serving kernels, or true 32-bit).
+it selects the whole path (bfloat16 serving kernels, or true 32-bit).  ``generate --logprobs`` prints every token's log probability
+and alternatives, ``--draft`` verifies drafts that the text itself suggests; ``score`` says how likely the tokens of a text are.
 """
 from __future__ import annotations
 
@@ -145,19 +146,45 @@ def cmd_generate(args) -> int:
         sys.stdout.flush()
         return False
 
+    more = {}
+    if args.logprobs is not None:
+        more["logprobs"] = args.logprobs
+    if args.draft:
+        from .engine import PromptLookup
+        more["drafter"] = PromptLookup(length=args.draft)
     prof = _profiler(args, eng)
     if prof is not None:
         with prof:
             out = eng.generate([ids], max_new_tokens=args.max_tokens, sampling=sampling, on_token=show, stats=stats,
-                               run_ahead=False)
+                               run_ahead=False, **more)
     else:
-        out = eng.generate([ids], max_new_tokens=args.max_tokens, sampling=sampling, on_token=show, stats=stats)
+        out = eng.generate([ids], max_new_tokens=args.max_tokens, sampling=sampling, on_token=show, stats=stats, **more)
     print()
+    for s in out[0].logprobs or []:
+        _show_score(s)
     _emit_profile(args, prof)
     print(f"prompt: {stats.prompt_tokens} tokens in {stats.prefill_seconds:.3f}s "
           f"({stats.prompt_tokens_per_sec:.1f} tok/s); decode: {stats.decode_tokens} tokens in "
           f"{stats.decode_seconds:.3f}s ({stats.decode_tokens_per_sec:.1f} tok/s); finished: {out[0].finish_reason}",
           file=sys.stderr)
+    return 0
+
+
+def _show_score(s) -> None:
+    top = "".join(f"  {t}:{lp:.4f}" for t, lp in s.top)
+    print(f"{s.token}  logprob {s.logprob:.4f}  entropy {s.entropy:.4f}{top}")
+
+
+def cmd_score(args) -> int:
+    import math
+    eng, entry, tmp = _open_engine(args, batch=1)
+    ids = _prompt_ids(args, eng.model.vocab)
+    scores = eng.score([ids], top=args.top)[0]
+    for s in scores:
+        _show_score(s)
+    if scores:
+        mean = sum(s.logprob for s in scores) / len(scores)
+        print(f"{len(scores)} tokens, mean log probability {mean:.4f}, perplexity {math.exp(min(-mean, 700.0)):.4f}", file=sys.stderr)
     return 0
 
 
@@ -234,8 +261,20 @@ def main(argv=None) -> int:
     g.add_argument("--top-p", type=float, default=None)
     g.add_argument("--top-k", type=int, default=None)
     g.add_argument("--seed", type=int, default=None)
+    g.add_argument("--logprobs", type=int, default=None, metavar="K",
+                   help="score every token: its log probability, the entropy and K alternatives (0 to 32)")
+    g.add_argument("--draft", type=int, default=0, metavar="N",
+                   help="verify drafts of up to N tokens that followed the text's last tokens before (the answer is the same)")
     _profile_args(g)
     g.set_defaults(fn=cmd_generate)
+
+    s = sub.add_parser("score", help="how likely every token of a text of token ids is after the ones before it")
+    _model_args(s)
+    s.add_argument("--prompt-ids", default=None, help="token ids, comma or space separated")
+    s.add_argument("--prompt-file", default=None, help="a file of token ids")
+    s.add_argument("--prompt-len", type=int, default=16, help="length of a synthetic text when no ids are given")
+    s.add_argument("--top", type=int, default=0, help="alternatives a token (0 to 32)")
+    s.set_defaults(fn=cmd_score)
 
     b = sub.add_parser("bench", help="prompt and decode throughput, greedy, stop tokens ignored")
     _model_args(b)

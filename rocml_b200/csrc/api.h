@@ -346,7 +346,7 @@ int rb_rglru_step(const float* u, int ld_u, const void* ra, const void* ri, int 
 
 // Attention of trees of drafted tokens over the paged cache (attention_tree.cu): sequence b's nodes are the rows cu_q[b] .. cu_q[b + 1], their keys
 // and values lie at the places kv_len[b] - n + j; row t sees the context (inside `window` of positions[t], and below `keep`) and the nodes whose
-// bits are set in visible[t] (int32 [tokens, words]).  shares: blocks that share a head's pages; rows_tile: 16, or 128 / group * group for
+// bits are set in visible[t] (int32 [tokens, words]).  shares: blocks that share a head's pages; rows_tile: 16 or 32, or 128 / group * group for
 // the tensor-core kernel.
 typedef struct RbTreeCall {
     const void *q, *k_cache, *v_cache;

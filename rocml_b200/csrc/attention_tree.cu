@@ -21,17 +21,18 @@
 #include "api.h"
 #include "per_device.h"
 #include "tree.cuh"
+#include <type_traits>
 
 using namespace rb_tree;
 
 namespace {
 // ---- any head size, both types, 32-bit multiply-adds ------------------------------------------------------------------
-// 128 threads, 16 rows by 64 keys a tile.  Keys and values come 64 dimensions at a time, as float32, through a ring of RING blocks of shared memory:
+// 128 threads, 8 RPT rows (16, or 32 where trees have more) by 64 keys a tile.  Keys and values come 64 dimensions at a time, as float32, through a ring of RING blocks of shared memory:
 // a tile is its blocks of keys, then its blocks of values, and RING - 1 blocks are asked for ahead of the one in use (32-bit rows by cp.async; staged through
-// registers a block waited for memory four times a tile: 10 us).  Thread (rg, kg), rg = t / 16, kg = t % 16, forms the scores of rows 2 rg, 2 rg + 1
-// against keys kg + 16 i, and the results of the same rows at dimensions 4 kg .. 4 kg + 3 of every block of 64: six 16-byte reads of shared
-// memory for 32 multiply-adds in both products.
-constexpr int SR = 16, SLD = 68;      // rows a tile; row stride of a staged [64][64] block (68 floats: 16-byte reads of 8 rows miss each other's banks)
+// registers a block waited for memory four times a tile: 10 us).  Thread (rg, kg), rg = t / 16, kg = t % 16, forms the scores of rows RPT rg .. RPT rg + RPT - 1
+// against keys kg + 16 i, and the results of the same rows at dimensions 4 kg .. 4 kg + 3 of every block of 64: RPT + 4 16-byte reads of shared
+// memory for 16 RPT multiply-adds in both products.
+constexpr int SLD = 68;               // row stride of a staged [64][64] block (68 floats: 16-byte reads of 8 rows miss each other's banks)
 constexpr int RING = 4;
 
 __device__ __forceinline__ void copy_async16(void* dst, const void* src, bool real) {
@@ -72,16 +73,17 @@ __device__ __forceinline__ void stage64(const T* src, int hd, int d0, int rows, 
     for (int i = 0; i < 8; ++i) rb::store4(dst + (r0 + 8 * i) * SLD + d, x[i]);
 }
 
-template <typename T, int BLOCKS>       // BLOCKS: blocks of 64 dimensions a head, 1, 2, 4 or 8
+template <typename T, int BLOCKS, int RPT>       // BLOCKS: blocks of 64 dimensions a head, 1, 2, 4 or 8
 __global__ void __launch_bounds__(128)
 attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out, long long o_stride,
                              const T* __restrict__ k_cache, const T* __restrict__ v_cache, const TreeArgs a) {
     rb::pdl_trigger();
     rb::pdl_wait();
+    constexpr int SR = 8 * RPT;
     extern __shared__ float smem[];
-    float* Qs = smem;                              // [16][64 BLOCKS]
+    float* Qs = smem;                              // [SR][64 BLOCKS]
     float* Ring = Qs + SR * 64 * BLOCKS;           // [RING][64][SLD]
-    float* Ps = Ring + RING * 64 * SLD;            // [16][SLD]
+    float* Ps = Ring + RING * 64 * SLD;            // [SR][SLD]
     int* pre = (int*)(Ps + SR * SLD);
     int* tl = pre + a.B + 1;
     const int kvh = blockIdx.y;
@@ -127,33 +129,38 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
             }
             Qs[i] = x;
         }
-        RowBits bits[2];
+        RowBits bits[RPT];
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-            if (2 * rg + r < rows) bits[r].load(a, s.q0 + (row0 + 2 * rg + r) / a.group);
-        float m[2] = {NEG_BIG, NEG_BIG}, l[2] = {0.f, 0.f}, o[BLOCKS][2][4];
+        for (int r = 0; r < RPT; ++r)
+            if (RPT * rg + r < rows) bits[r].load(a, s.q0 + (row0 + RPT * rg + r) / a.group);
+        float m[RPT], l[RPT], o[BLOCKS][RPT][4];
 #pragma unroll
-        for (int c = 0; c < BLOCKS; ++c)
+        for (int r = 0; r < RPT; ++r) {
+            m[r] = NEG_BIG;
+            l[r] = 0.f;
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
+            for (int c = 0; c < BLOCKS; ++c)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[c][r][e] = 0.f;
+        }
         int block = 0;
         for (int j = p0; j < p1; ++j) {
             const int key0 = tile_of(s, j) * PAGE;
-            float sc[2][4] = {};
+            // a tile inside the context that every row sees whole needs no mask (no position is behind the sequence's last)
+            const bool whole_tile = key0 + PAGE <= s.ctx && (a.window == 0 || key0 >= s.len - a.window || key0 + PAGE <= a.keep);
+            float sc[RPT][4] = {};
 #pragma unroll 1
             for (int c = 0; c < BLOCKS; ++c) {
                 const float* Ks = arrive(block++);
 #pragma unroll 4
                 for (int d = 0; d < 64; d += 4) {
-                    float qa[2][4], kb[4][4];
+                    float qa[RPT][4], kb[4][4];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) rb::load4(Qs + (2 * rg + r) * 64 * BLOCKS + c * 64 + d, qa[r]);
+                    for (int r = 0; r < RPT; ++r) rb::load4(Qs + (RPT * rg + r) * 64 * BLOCKS + c * 64 + d, qa[r]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) rb::load4(Ks + (kg + 16 * i) * SLD + d, kb[i]);
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
+                    for (int r = 0; r < RPT; ++r)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -161,8 +168,9 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const unsigned long long seen = 2 * rg + r < rows ? bits[r].seen(a, s.ctx, s.n, key0) : 0ull;
+            for (int r = 0; r < RPT; ++r) {
+                unsigned long long seen = ~0ull;
+                if (!whole_tile) seen = RPT * rg + r < rows ? bits[r].seen(a, s.ctx, s.n, key0) : 0ull;
                 float mx = NEG_BIG;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -179,7 +187,7 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
                 for (int i = 0; i < 4; ++i) {
                     const float p = exp2f(sc[r][i] - m_new);
                     sum += p;
-                    Ps[(2 * rg + r) * SLD + kg + 16 * i] = p;
+                    Ps[(RPT * rg + r) * SLD + kg + 16 * i] = p;
                 }
                 l[r] = l[r] * alpha + sum;         // (each thread its own keys; joined at the end)
 #pragma unroll
@@ -187,35 +195,39 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[c][r][e] *= alpha;
             }
-#pragma unroll
-            for (int c = 0; c < BLOCKS; ++c) {
-                const float* Vs = arrive(block++);          // (its barrier also makes Ps whole)
+            // What a row does not see may hold anything, NaN too: in a masked tile a weight of zero takes no part.
+            auto add_values = [&](float (&oc)[RPT][4], const float* Vs, auto masked) {
 #pragma unroll 4
                 for (int key = 0; key < 64; key += 4) {
-                    float pa[2][4], vb[4][4];
+                    float pa[RPT][4], vb[4][4];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) rb::load4(Ps + (2 * rg + r) * SLD + key, pa[r]);
+                    for (int r = 0; r < RPT; ++r) rb::load4(Ps + (RPT * rg + r) * SLD + key, pa[r]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) rb::load4(Vs + (key + i) * SLD + 4 * kg, vb[i]);
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
+                    for (int r = 0; r < RPT; ++r)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (pa[r][i] != 0.f) {       // (what a row does not see may hold anything, NaN too)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) o[c][r][e] = fmaf(pa[r][i], vb[i][e], o[c][r][e]);
-                            }
+                            for (int e = 0; e < 4; ++e)
+                                if (!masked || pa[r][i] != 0.f) oc[r][e] = fmaf(pa[r][i], vb[i][e], oc[r][e]);
                 }
+            };
+#pragma unroll
+            for (int c = 0; c < BLOCKS; ++c) {
+                const float* Vs = arrive(block++);          // (its barrier also makes Ps whole)
+                if (whole_tile) add_values(o[c], Vs, std::false_type());
+                else add_values(o[c], Vs, std::true_type());
             }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         const bool whole = p0 == 0 && p1 == s.tiles;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < RPT; ++r) {
 #pragma unroll
             for (int w = 8; w > 0; w >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
-            if (2 * rg + r >= rows) continue;
-            const int row = row0 + 2 * rg + r, node = row / a.group, head = kvh * a.group + row % a.group;
+            if (RPT * rg + r >= rows) continue;
+            const int row = row0 + RPT * rg + r, node = row / a.group, head = kvh * a.group + row % a.group;
             if (whole) {
                 const float sink = (a.sinks ? a.sinks[head] : a.sink) * LOG2E;
                 float f = 1.f, total = l[r];
@@ -232,7 +244,7 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
                     for (int e = 0; e < 4; ++e)
                         if (c * 64 + 4 * kg + e < a.hd) dst[c * 64 + 4 * kg + e] = rb::from_f32<T>(o[c][r][e] * inv);
             } else {
-                const size_t place = ((size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * a.nkv + kvh) * a.rows_tile + 2 * rg + r;
+                const size_t place = ((size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * a.nkv + kvh) * a.rows_tile + RPT * rg + r;
                 if (kg == 0) { a.part_ml[place * 2] = m[r]; a.part_ml[place * 2 + 1] = l[r]; }
 #pragma unroll
                 for (int c = 0; c < BLOCKS; ++c)
@@ -393,11 +405,11 @@ attention_tree_merge_rows_kernel(__nv_bfloat16* __restrict__ out, long long o_st
     }
 }
 
-template <typename T, int BLOCKS>
+template <typename T, int BLOCKS, int RPT>
 int launch_simple(const void* q, long long q_stride, void* out, long long o_stride, const void* k, const void* v, const TreeArgs& a,
                   cudaStream_t stream) {
-    const size_t smem = (SR * 64 * BLOCKS + RING * 64 * SLD + SR * SLD) * sizeof(float) + (2 * a.B + 1) * sizeof(int);
-    auto kernel = attention_tree_simple_kernel<T, BLOCKS>;
+    const size_t smem = (8 * RPT * 64 * BLOCKS + RING * 64 * SLD + 8 * RPT * SLD) * sizeof(float) + (2 * a.B + 1) * sizeof(int);
+    auto kernel = attention_tree_simple_kernel<T, BLOCKS, RPT>;
     static rb::PerDevice<int> allowed;
     int device;
     cudaError_t e = cudaGetDevice(&device);
@@ -415,10 +427,15 @@ int launch_simple(const void* q, long long q_stride, void* out, long long o_stri
 template <typename T>
 int launch_any(const void* q, long long q_stride, void* out, long long o_stride, const void* k, const void* v, const TreeArgs& a,
                cudaStream_t stream) {
-    if (a.hd <= 64) return launch_simple<T, 1>(q, q_stride, out, o_stride, k, v, a, stream);
-    if (a.hd <= 128) return launch_simple<T, 2>(q, q_stride, out, o_stride, k, v, a, stream);
-    if (a.hd <= 256) return launch_simple<T, 4>(q, q_stride, out, o_stride, k, v, a, stream);
-    return launch_simple<T, 8>(q, q_stride, out, o_stride, k, v, a, stream);
+    if (a.rows_tile == 32) {                    // (32 rows of more than 256 dimensions do not fit a thread's registers)
+        if (a.hd <= 64) return launch_simple<T, 1, 4>(q, q_stride, out, o_stride, k, v, a, stream);
+        if (a.hd <= 128) return launch_simple<T, 2, 4>(q, q_stride, out, o_stride, k, v, a, stream);
+        return a.hd <= 256 ? launch_simple<T, 4, 4>(q, q_stride, out, o_stride, k, v, a, stream) : RB_ERR_BAD_SIZE;
+    }
+    if (a.hd <= 64) return launch_simple<T, 1, 2>(q, q_stride, out, o_stride, k, v, a, stream);
+    if (a.hd <= 128) return launch_simple<T, 2, 2>(q, q_stride, out, o_stride, k, v, a, stream);
+    if (a.hd <= 256) return launch_simple<T, 4, 2>(q, q_stride, out, o_stride, k, v, a, stream);
+    return launch_simple<T, 8, 2>(q, q_stride, out, o_stride, k, v, a, stream);
 }
 
 template <typename T>
@@ -434,7 +451,7 @@ int launch_merge(void* out, long long o_stride, const TreeArgs& a, cudaStream_t 
 }
 }  // namespace
 
-// rows_tile: 16, the plain kernel; 128 / group * group, the tensor-core kernel (attention_tree_tc5.cu), which takes aligned rows only.  work (shares > 1,
+// rows_tile: 16 or 32 (heads of up to 256), the plain kernel; 128 / group * group, the tensor-core kernel (attention_tree_tc5.cu), which takes aligned rows only.  work (shares > 1,
 // 16-byte aligned): 2 shares * nkv * rows_tile * (hd + 2) floats, then nkv * min(shares - 1, n_seqs * tiles of rows of max_nodes nodes) entries
 // of four ints.
 extern "C" int rb_attention_tree(const RbTreeCall* call, void* stream) {
@@ -447,7 +464,7 @@ extern "C" int rb_attention_tree(const RbTreeCall* call, void* stream) {
     if (x.dtype != RB_F32 && x.dtype != RB_BF16) return RB_ERR_BAD_DTYPE;
     if ((uintptr_t)x.work & 15) return RB_ERR_BAD_ALIGN;
     const int group = x.nq / x.nkv;
-    const bool tc5 = x.rows_tile != SR;
+    const bool tc5 = x.rows_tile != 16 && x.rows_tile != 32;
     if (tc5 && (x.dtype != RB_BF16 || (x.hd != 64 && x.hd != 128 && x.hd != 256) || group > 128 || x.rows_tile != 128 / group * group)) return RB_ERR_BAD_SIZE;
     TreeArgs a{};
     a.block_table = x.block_table; a.max_pages = x.max_pages; a.seq_slot = x.seq_slot; a.cu_q = x.cu_q; a.kv_len = x.kv_len;

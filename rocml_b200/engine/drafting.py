@@ -104,25 +104,36 @@ def generate_drafted(engine, requests: Sequence[Request], drafter: Drafter, defa
                     return False
             return True
 
-        first = True
-        while live:
-            t0 = time.perf_counter()
-            before = sum(len(s["out"]) for s in live)
-            if first:
-                sampled = [[t] for t in engine.run([s["slot"] for s in live], [s["history"] for s in live], [s["req"].sampling for s in live],
-                                                   [s["rng"] for s in live], [s["history"] for s in live])]
-            else:
-                entries = [_entry(s["slot"], s["history"], drafter, s["need"] - len(s["history"]) + 1) for s in live]
-                sampled = engine.verify(entries, [s["req"].sampling for s in live], [s["rng"] for s in live], [s["history"] for s in live])
-            running = live
-            live = [s for s, tokens in zip(running, sampled) if take(s, tokens)]
-            dt = time.perf_counter() - t0
-            stats.step_batch_sizes.append(len(running))
-            if first:
-                stats.prefill_seconds += dt
-                stats.prompt_tokens += sum(len(s["req"].prompt) for s in running)
-                first = False
-            else:
-                stats.decode_seconds += dt
-                stats.decode_tokens += sum(len(s["out"]) for s in running) - before
+        try:
+            _run_batch(engine, live, drafter, take, stats)
+        except BaseException:
+            for s in live:                    # (a drafter may fail: the sequences that were running give their slots back)
+                if results[s["i"]] is None:
+                    engine.release(s["slot"])
+            raise
     return results
+
+
+def _run_batch(engine, live, drafter, take, stats) -> None:
+    """Prompts, then drafts until every sequence has ended."""
+    first = True
+    while live:
+        t0 = time.perf_counter()
+        before = sum(len(s["out"]) for s in live)
+        if first:
+            sampled = [[t] for t in engine.run([s["slot"] for s in live], [s["history"] for s in live], [s["req"].sampling for s in live],
+                                               [s["rng"] for s in live], [s["history"] for s in live])]
+        else:
+            entries = [_entry(s["slot"], s["history"], drafter, s["need"] - len(s["history"]) + 1) for s in live]
+            sampled = engine.verify(entries, [s["req"].sampling for s in live], [s["rng"] for s in live], [s["history"] for s in live])
+        running = live
+        live = [s for s, tokens in zip(running, sampled) if take(s, tokens)]
+        dt = time.perf_counter() - t0
+        stats.step_batch_sizes.append(len(running))
+        if first:
+            stats.prefill_seconds += dt
+            stats.prompt_tokens += sum(len(s["req"].prompt) for s in running)
+            first = False
+        else:
+            stats.decode_seconds += dt
+            stats.decode_tokens += sum(len(s["out"]) for s in running) - before

@@ -893,25 +893,25 @@ def sample(logits: torch.Tensor, n: int, rows: torch.Tensor, history: Optional[t
 
 TREE_MAX_NODES = 256       # nodes a tree holds at most (rows of 8 words of bits)
 TREE_MAX_SEQS = 1024       # sequences a call takes
-_TREE_ROWS = 16            # rows of a tile of attention_tree's plain kernel
 
 
-def _here(what: str, *tensors) -> None:
-    """The launch goes to the current device's current stream: every tensor must live there."""
-    device = tensors[0].get_device()
-    for t in tensors:
+def _ints_here(what: str, ints, others) -> None:
+    """The launch goes to the current device's current stream: every tensor must live there; ``ints`` are contiguous int32."""
+    device = others[0].get_device() if others else ints[0].get_device()
+    i32 = torch.int32
+    for t in ints:
+        if t is not None:
+            if t.dtype is not i32 or not t.is_contiguous():
+                raise KernelError(f"{what}: ids, lengths, tables and bits must be contiguous int32 tensors")
+            if t.get_device() != device:
+                raise KernelError(f"{what}: every tensor must live on one device")
+    for t in others:
         if t is not None and t.get_device() != device:
             raise KernelError(f"{what}: every tensor must live on one device")
     if device < 0:
         raise KernelError(f"{what}: arguments must live on a CUDA device; there is no CPU path")
     if device != torch._C._cuda_getDevice():
         raise KernelError(f"{what}: its tensors live on device {device}, which is not the current one")
-
-
-def _ints(what: str, *tensors) -> None:
-    for t in tensors:
-        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()):
-            raise KernelError(f"{what}: ids, lengths, tables and bits must be contiguous int32 tensors")
 
 
 def _tree_sizes(what: str, visible, cu_q, n_seqs: int, max_nodes: int):
@@ -936,6 +936,20 @@ def tree_shares(pairs: int, rows: int, nkv: int, slots: int) -> int:
     sixteen of a tile's ``rows``: what a block leaves to be joined is as much as that to write and read again.  (256 rows over 4,164 keys, 8 heads,
     in blocks of 3.5 pages 21.5 us, of 8 pages 18.5; 16 rows over 709 keys in blocks of one page 10.7, of two 11.6.)"""
     return max(1, min(slots // nkv if nkv <= slots else -(-4 * slots // nkv), pairs // max(1, rows // 16)))
+
+
+@functools.lru_cache(maxsize=4096)
+def _tree_plan(tensor_cores: bool, n_seqs: int, max_nodes: int, group: int, nkv: int, hd: int, n_pages: int, device: int):
+    """(rows of a tile, blocks that share a head's work, 32-bit words of work space) of a call of attention_tree, from its sizes."""
+    slots = _decode_slots(device) // 3 * 2             # two blocks a multiprocessor
+    if tensor_cores:
+        rows_tile = 128 // group * group               # whole nodes in 128 rows
+        slots = slots if hd <= 128 else slots // 2
+    else:
+        rows_tile = 32 if max_nodes * group > 16 and hd <= 256 else 16
+    units = n_seqs * -(-max_nodes * group // rows_tile)
+    shares = tree_shares(n_pages * units, min(rows_tile, max_nodes * group), nkv, slots)
+    return rows_tile, shares, 0 if shares == 1 else 2 * shares * nkv * rows_tile * (hd + 2) + 4 * nkv * min(shares - 1, units)
 
 
 @_profiled(lambda a, facts: _attention_cost(a, facts))
@@ -969,27 +983,18 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         raise KernelError("attention_tree: scale is positive, window, keep and softcap are not negative, a window comes with positions")
     if seq_slot.numel() < n_seqs or kv_len.numel() < n_seqs or block_table.dim() != 2:
         raise KernelError("attention_tree: seq_slot, kv_len and block_table do not fit")
-    _ints("attention_tree", block_table, seq_slot, cu_q, kv_len, visible, positions)
-    _here("attention_tree", q, out, k_cache, v_cache, block_table, seq_slot, cu_q, kv_len, visible, positions)
+    _ints_here("attention_tree", (block_table, seq_slot, cu_q, kv_len, visible, positions), (q, out, k_cache, v_cache))
     if n_seqs == 0:
         return
     one_sink, sinks = _sink(sink, nq)
     max_pages = block_table.shape[1]
     longest = max_pages if max_kv_len is None else max(1, min(max_pages, (int(max_kv_len) + PAGE - 1) // PAGE))
     device = q.device
-    group = nq // nkv
-    slots = _decode_slots(device) // 3 * 2             # two blocks a multiprocessor
-    rows_tile = _TREE_ROWS
     pointers = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
-    if dtype is torch.bfloat16 and hd in (64, 128, 256) and group <= 128 and not \
-            ((pointers[0] | pointers[1] | pointers[2] | pointers[3]) & 15 or (q_stride | o_stride) & 7):
-        rows_tile = 128 // group * group               # the tensor-core kernel: whole nodes in 128 rows
-        slots = slots if hd <= 128 else slots // 2
-    units = n_seqs * -(-max_nodes * group // rows_tile)
-    shares = tree_shares(longest * units, min(rows_tile, max_nodes * group), nkv, slots)
-    work = None
-    if shares > 1:
-        work = torch.empty(2 * shares * nkv * rows_tile * (hd + 2) + 4 * nkv * min(shares - 1, units), dtype=torch.float32, device=device)
+    tensor_cores = dtype is torch.bfloat16 and hd in (64, 128, 256) and nq <= 128 * nkv and not \
+        ((pointers[0] | pointers[1] | pointers[2] | pointers[3]) & 15 or (q_stride | o_stride) & 7)
+    rows_tile, shares, words_of_work = _tree_plan(tensor_cores, n_seqs, max_nodes, nq // nkv, nkv, hd, longest, device.index)
+    work = torch.empty(words_of_work, dtype=torch.float32, device=device) if words_of_work else None
     call = _TREE_CALL.pack(
         *pointers, block_table.data_ptr(), seq_slot.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
         0 if positions is None else positions.data_ptr(), sinks or 0, 0 if work is None else work.data_ptr(), status_word(device).data_ptr(),
@@ -1032,8 +1037,8 @@ def tree_accept(token_ids: torch.Tensor, parents: torch.Tensor, visible: torch.T
         layers, n_pages, nkv = k.shape[0], k.shape[1], k.shape[2]
         esz = k.element_size()
         row_bytes, max_pages = k.shape[4] * esz, block_table.shape[1]
-    _ints("tree_accept", token_ids, parents, visible, sampled, cu_q, path, counts, next_token, seq_slot, kv_len, block_table)
-    _here("tree_accept", token_ids, parents, visible, sampled, cu_q, path, counts, next_token, seq_slot, kv_len, block_table, k, v)
+    _ints_here("tree_accept", (token_ids, parents, visible, sampled, cu_q, path, counts, next_token, seq_slot, kv_len, block_table),
+               () if k is None else (k, v))
     if n_seqs == 0:
         return
     pointer = lambda t: None if t is None else t.data_ptr()
@@ -1088,8 +1093,7 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor], logprobs: 
             raise KernelError(f"token_logprobs: top_ids int32 and top_logprobs float32 [n, k], contiguous, k at most {LOGPROBS_MAX_TOP} and the vocabulary")
     if n == 0:
         return
-    _ints("token_logprobs", ids, top_ids)
-    _here("token_logprobs", logits, ids, logprobs, entropy, top_logprobs, top_ids)
+    _ints_here("token_logprobs", (ids, top_ids), (logits, logprobs, entropy, top_logprobs))
     pointer = lambda t: None if t is None else t.data_ptr()
     rc = _lib().rb_token_logprobs(
         logits.data_ptr(), dtype_code(logits.dtype), logits.stride(0), n, V, pointer(ids), m, pointer(logprobs), pointer(entropy),

@@ -540,10 +540,10 @@ def paged_attention(q, out, batch, k_cache, v_cache, block_table, nq, nkv, hd, s
     A step of trees of drafted tokens (``batch.tree``): every node sees its sequence's context and its ancestors.
     ``cross`` (n > 1, the cache's own number of key/value heads): every query head's weights are applied to the values of
     every stored head; nkv = n * n then counts (key head, value head) pairs and nq = n * query heads the results."""
-    if batch.tree is not None:
+    t = getattr(batch, "tree", None)
+    if t is not None:
         if cross > 1 or window < 0:
             raise ConfigError("attention: mixed heads and masks by blocks of positions do not take trees of drafted tokens")
-        t = batch.tree
         kernels.attention_tree(q, out, k_cache, v_cache, block_table, batch.seq_slot, batch.cu_q, batch.kv_len, t.visible, batch.n_seqs,
                                t.max_nodes, nq, nkv, hd, scale, max_kv_len=batch.max_kv_len, positions=t.positions, window=window, keep=keep,
                                sink=sink, softcap=softcap)

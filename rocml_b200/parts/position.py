@@ -114,7 +114,8 @@ class RotaryNeox(PositionEncoding):
         from .. import kernels
         key = ("rope", self.rot_dim, self.theta, self.scaling, self.ramp_scaling)      # layers with the same angles share the table
         if key not in batch.scratch:
-            batch.scratch[key] = kernels.rope_table(batch.angle_positions, self.inv_freq, batch.n_tokens, self.magnitude)
+            positions = getattr(batch, "angle_positions", batch.positions)
+            batch.scratch[key] = kernels.rope_table(positions, self.inv_freq, batch.n_tokens, self.magnitude)
         return batch.scratch[key]
 
 

@@ -158,8 +158,10 @@ def test_drafted_generation_refuses():
         generate_drafted(Fake(), [Request([])], PromptLookup())
     with pytest.raises(RocmlError, match="do not come with drafts"):
         generate_drafted(Fake(), [Request([1], logprobs=2)], PromptLookup())
+    fake = Fake()
     with pytest.raises(RocmlError, match="3 tokens and 2 parents"):
-        generate_drafted(Fake(), [Request([1, 2, 3], 5)], lambda h: ([1, 2, 3], [-1, 0]))
+        generate_drafted(fake, [Request([1, 2, 3], 5), Request([4], 1), Request([5], 5)], lambda h: ([1, 2, 3], [-1, 0]))
+    assert not fake.text                      # every slot is back
 
 
 class Scoring(Fake):
