@@ -117,18 +117,29 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
             return Ring + i % RING * 64 * SLD;
         };
         __syncthreads();
+        // the rows' queries, sixteen threads a row; 32-bit rows on 16 bytes in the first group of copies
+        const bool q16 = sizeof(T) == 4 && a.hd % 4 == 0 && q_stride % 4 == 0 && ((uintptr_t)q & 15) == 0;
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const int r = rg + 8 * i, row = row0 + r, node = row / a.group, h = row - node * a.group;
+            const T* src = q + (size_t)(s.q0 + (r < rows ? node : 0)) * q_stride + (size_t)(kvh * a.group + (r < rows ? h : 0)) * a.hd;
+#pragma unroll
+            for (int c = 0; c < BLOCKS; ++c) {
+                const int d = c * 64 + 4 * kg;
+                float* dst = Qs + r * 64 * BLOCKS + d;
+                if (q16) {
+                    const bool real = r < rows && d < a.hd;
+                    copy_async16(dst, real ? src + d : src, real);
+                } else {
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = r < rows && d + e < a.hd ? rb::to_f32(__ldg(src + d + e)) : 0.f;
+                    rb::store4(dst, x);
+                }
+            }
+        }
 #pragma unroll 1
         for (int i = 0; i < RING - 1; ++i) fetch(i);
-#pragma unroll 8
-        for (int i = threadIdx.x; i < SR * 64 * BLOCKS; i += 128) {
-            const int r = i / (64 * BLOCKS), d = i % (64 * BLOCKS);
-            float x = 0.f;
-            if (r < rows && d < a.hd) {
-                const int node = (row0 + r) / a.group, h = (row0 + r) - node * a.group;
-                x = rb::to_f32(__ldg(q + (size_t)(s.q0 + node) * q_stride + (size_t)(kvh * a.group + h) * a.hd + d));
-            }
-            Qs[i] = x;
-        }
         RowBits bits[RPT];
 #pragma unroll
         for (int r = 0; r < RPT; ++r)

@@ -123,11 +123,13 @@ def test_confirmed_nodes_by_bits_are_the_walk(seed):
 
 
 def test_shares_fill_the_device_and_never_outnumber_the_pages():
-    assert kernels.tree_shares(200, 64, 8, 296) == 37
-    assert kernels.tree_shares(200, 128, 8, 296) == 25
-    assert kernels.tree_shares(3, 16, 8, 296) == 3
-    assert kernels.tree_shares(320, 5, 1000, 296) == 2
-    assert kernels.tree_shares(1, 128, 5000, 296) == 1
+    assert kernels.tree_shares(200, 1, 64, 8, 296) == 37
+    assert kernels.tree_shares(200, 1, 128, 8, 296) == 25
+    assert kernels.tree_shares(14, 14, 128, 8, 296) == 14
+    assert kernels.tree_shares(324, 36, 26, 8, 296) == 36 and kernels.tree_shares(324, 20, 26, 8, 296) == 37
+    assert kernels.tree_shares(3, 1, 16, 8, 296) == 3
+    assert kernels.tree_shares(320, 32, 5, 1000, 296) == 2
+    assert kernels.tree_shares(1, 1, 128, 5000, 296) == 1
 
 
 def _attention(**change):
