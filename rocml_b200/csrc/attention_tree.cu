@@ -347,6 +347,7 @@ attention_tree_merge_rows_kernel(__nv_bfloat16* __restrict__ out, long long o_st
     rb::pdl_trigger();
     rb::pdl_wait();
     __shared__ float part[JOIN_WARPS][JOIN_DIMS][33], tops[JOIN_WARPS][32], sums[JOIN_WARPS][32];
+    __shared__ long long offset[32];
     const int kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row_blocks = (a.rows_tile + 31) / 32, r0 = blockIdx.x % row_blocks * 32;
     const int4 note = *note_of(a, kvh, blockIdx.z);
@@ -394,24 +395,29 @@ attention_tree_merge_rows_kernel(__nv_bfloat16* __restrict__ out, long long o_st
 #pragma unroll
         for (int d = 0; d < JOIN_DIMS; ++d) part[warp][d][lane] = acc[d];
         __syncthreads();
+        // what each way's part of a row is multiplied by, a lane a row (every block of dimensions has the same maxima and sums)
+        if (warp == 0) {
+            const int row = note.y + r0 + lane, node = row / a.group, head = kvh * a.group + row - node * a.group;
+            const float sink = (a.sinks ? a.sinks[min(head, a.nq - 1)] : a.sink) * LOG2E;
+            float m = rb::has_sink(sink) ? sink : NEG_BIG;
+            for (int w = 0; w < ways; ++w) m = fmaxf(m, tops[w][lane]);
+            float l = rb::has_sink(sink) ? exp2f(sink - m) : 0.f;
+            for (int w = 0; w < ways; ++w) l = fmaf(sums[w][lane], exp2f(tops[w][lane] - m), l);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            for (int w = 0; w < ways; ++w) sums[w][lane] = exp2f(tops[w][lane] - m) * inv;
+            offset[lane] = (long long)(note.x + node) * o_stride + (long long)head * a.hd + base;
+        }
+        __syncthreads();
         // two neighbouring dimensions of a row a thread and round
         for (int i = threadIdx.x; i < chunks * (JOIN_DIMS / 2) * 32; i += 32 * JOIN_WARPS) {
             const int d = i % (JOIN_DIMS / 2) * 2, rr = i / (JOIN_DIMS / 2) % 32, chunk = i / (JOIN_DIMS / 2 * 32), w0 = chunk * ways;
             if (r0 + rr >= note.z || base + chunk * JOIN_DIMS >= a.hd) continue;
-            const int row = note.y + r0 + rr, node = row / a.group, head = kvh * a.group + row % a.group;
-            const float sink = (a.sinks ? a.sinks[head] : a.sink) * LOG2E;
-            float m = rb::has_sink(sink) ? sink : NEG_BIG;
-            for (int w = w0; w < w0 + ways; ++w) m = fmaxf(m, tops[w][rr]);
-            float l = rb::has_sink(sink) ? exp2f(sink - m) : 0.f, y0 = 0.f, y1 = 0.f;
-            for (int w = w0; w < w0 + ways; ++w) {
-                const float f = exp2f(tops[w][rr] - m);
-                l = fmaf(sums[w][rr], f, l);
-                y0 = fmaf(part[w][d][rr], f, y0);
-                y1 = fmaf(part[w][d + 1][rr], f, y1);
+            float y0 = 0.f, y1 = 0.f;
+            for (int w = 0; w < ways; ++w) {
+                y0 = fmaf(part[w0 + w][d][rr], sums[w][rr], y0);
+                y1 = fmaf(part[w0 + w][d + 1][rr], sums[w][rr], y1);
             }
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            *reinterpret_cast<__nv_bfloat162*>(out + (size_t)(note.x + node) * o_stride + (size_t)head * a.hd + base + chunk * JOIN_DIMS + d) =
-                __floats2bfloat162_rn(y0 * inv, y1 * inv);
+            *reinterpret_cast<__nv_bfloat162*>(out + offset[rr] + chunk * JOIN_DIMS + d) = __floats2bfloat162_rn(y0, y1);
         }
     }
 }

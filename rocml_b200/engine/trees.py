@@ -76,7 +76,7 @@ class TreeSteps:
             raise ConfigError("this model keeps more than keys and values a sequence, or masks that have no form for trees of drafted tokens")
         self.engine = engine
         # (a step's logits, one row a node, stay within the head room of the engine's memory budget)
-        self.max_nodes = min(engine.max_step_tokens, max(MAX_NODES, engine.cache.max_slots))
+        self.max_nodes = min(engine.max_step_tokens, max(2 * MAX_NODES, engine.cache.max_slots))
         self._buffers = {}
         self._sampler = None
 
