@@ -8,6 +8,9 @@
 // memory, at this multiprocessor's part of the bandwidth, about 2,900, so up to 128 rows the reads decide and the rows are free.  Two blocks share a
 // multiprocessor (up to heads of 128): one's products and softmax run beside the other's.
 //
+// Measured: 100,003 keys on 8 heads, 64 rows, 66 us = 6.2 TB/s; 32 sequences of up to 12,100 keys and trees of 9 to 33 nodes, 4 query heads a
+// key/value head, 133 us for 815 MB; a block alone on its multiprocessor 0.95 us a tile, waiting for the ring of two pages.
+//
 // A share may hold pieces of several sequences, one after the other: the rings and the two score buffers run on, Q and O are handed over at
 // the pieces' ends (q_empty, o_free).  P is rounded to bfloat16 for its product (the sums are of the 32-bit values); everything
 // else is 32-bit until the result.
@@ -85,7 +88,6 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                           int* __restrict__ status) {
     using Z = Sizes<HD>;
     constexpr int HALVES = Z::HALVES, Q_HALF = Z::Q_HALF, KV_HALF = Z::KV_HALF, KV_TILE = Z::KV_TILE, STAGES = Z::STAGES;
-    rb::pdl_trigger();
     rb::pdl_wait();
     extern __shared__ uint8_t smem_raw[];
     uint8_t* Qs = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -122,6 +124,9 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     tc_fence_before();
     const int extra = prefix_tiles(a, pre, tl);              // (ends with a block-wide barrier)
     tc_fence_after();
+    // Only now may later kernels be scheduled: products take their tensor memory before they wait for this kernel, and one that took a
+    // multiprocessor's columns ahead of a block of this grid would wait for it for good.
+    rb::pdl_trigger();
     const uint32_t tmem_base = bar->tmem_slot;
     Pieces pieces(pre, a.B, a.shares, blockIdx.x, extra);
     int b, mt, p0, p1;

@@ -11,6 +11,8 @@
 // row) are read again, all at once.  Keys are 64-bit whole numbers that order like (value, -index); places are found by counting the keys ahead.
 //
 // A row is read by one block or by the blocks of a cluster, which meet in the first one's shared memory.
+//
+// Memory bounds it where there are rows enough (2,047 rows of 151,936: 190 us, 6.5 TB/s); one row with 20 alternatives takes 7.6 us, 4.5 of them without.
 #include "common.cuh"
 #include "api.h"
 #include "per_device.h"
