@@ -173,6 +173,43 @@ def test_verify_in_graphs_and_in_pieces(folders):
     assert [small.length(x) for x in s] == [20, 20]
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_trees_behind_nothing_and_up_to_the_last_place(folders, dtype):
+    """A sequence without a context, ordinary steps between verified ones, a tree whose nodes end at the context's last place; one more is refused."""
+    from rocml_b200 import ContextOverflow, Engine, SamplingParams, StepEntry, TreeEntry
+    vocab = vocab_of("D")
+    eng = Engine.from_folder(folders("D"), dtype=dtype, max_tokens=192, max_slots=2, max_seq_len=128)
+    greedy = [SamplingParams()]
+    ids = prompt(3, 4, vocab)
+    slot, other = eng.new_sequence(), eng.new_sequence()
+    tree = TreeEntry(slot, [ids[0], ids[1], ids[2], ids[1]], [-1, 0, 1, 0])
+    lone = eng.step([StepEntry(other, ids[:3], [0, 1, 2])])
+    got = eng.tree_logits([tree])
+    assert rel_err(got[:3], lone) < 2 * TOL[dtype] and rel_err(got[3:], lone[1:2]) < 2 * TOL[dtype]
+    text = [ids[0]]
+    while len(text) < 120:
+        # the token that an ordinary step would draw next is among the guesses every third time
+        old = eng.length(slot)
+        assert old == len(text) - 1
+        want = int(eng.tree_logits([TreeEntry(slot, [text[-1]], [-1])]).argmax())
+        guess = want if len(text) % 3 == 0 else (want + 1) % vocab
+        new = eng.verify([TreeEntry(slot, [text[-1], (want + 2) % vocab, guess], [-1, 0, 0])], greedy)[0]
+        assert new[0] == want and len(new) == (2 if guess == want else 1)
+        text += new
+        if len(text) % 5 == 0:
+            logits = eng.step([StepEntry(slot, [text[-1]], [0])])
+            text.append(int(logits.argmax()))
+    eng.release(other)
+    old = eng.length(slot)
+    n = 128 - old
+    fits = TreeEntry(slot, [text[-1]] + [1] * (n - 1), [-1] + [0] * (n - 1))
+    assert eng.tree_logits([fits]).shape[0] == n
+    with pytest.raises(ContextOverflow):
+        eng.verify([TreeEntry(slot, fits.tokens + [1], fits.parents + [0])], greedy)
+    assert eng.length(slot) == old
+    eng.cache.check_invariants()
+
+
 def test_models_that_keep_more_than_keys_and_values_refuse_trees(tmp_path):
     from rocml_b200 import ConfigError, Engine, TreeEntry
     from tiny_models import TIBENEX, write_tibenex
