@@ -12,8 +12,8 @@
 // key/value head, 133 us for 815 MB; a block alone on its multiprocessor 0.95 us a tile, waiting for the ring of two pages.
 //
 // A share may hold pieces of several sequences, one after the other: the rings and the two score buffers run on, Q and O are handed over at
-// the pieces' ends (q_empty, o_free).  P is rounded to bfloat16 for its product (the sums are of the 32-bit values); everything
-// else is 32-bit until the result.
+// the pieces' ends (q_empty, o_free).  P is rounded to bfloat16 for its product, and the row's sum is that of the rounded weights;
+// everything else is 32-bit until the result.
 #include "api.h"
 #include "per_device.h"
 #include "sm100.cuh"
@@ -269,6 +269,11 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                 const bool whole_tile = key0 + BK <= s.ctx && (a.window == 0 || key0 >= s.len - a.window || key0 + BK <= a.keep);
                 unsigned long long seen = ~0ull;
                 bool spoiled = false;
+                // This wait comes before the one for V: scores of this tile say that the product of the tile before last is done, and so that the V before
+                // this one in its stage has landed.  Without that the wait for V could take that one's phase for this one's.
+                alive = __all_sync(0xffffffffu, wait_or_abort(&bar->s_full[buf], (it >> 1) & 1, &bar->abort_flag));
+                if (!alive) break;
+                tc_fence_after();
                 if (!whole_tile) {
                     seen = row_here ? bits.seen(a, s.ctx, s.n, key0) : 0ull;
                     // Weights of zero still multiply what lies in V: rows past the sequence's end are stale, and a value that is not finite
@@ -308,9 +313,6 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                     spoiled = (seen & (((unsigned long long)bad[1] << 32) | bad[0])) != 0;
                     ++checks;
                 }
-                alive = __all_sync(0xffffffffu, wait_or_abort(&bar->s_full[buf], (it >> 1) & 1, &bar->abort_flag));
-                if (!alive) break;
-                tc_fence_after();
                 if (warp_here) {
                     float sv[BK];
                     tmem_ld64(lane_base + buf * BK, sv);
@@ -362,10 +364,12 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                         for (int e = 0; e < 32; e += 2) {
                             float x0, x1;
                             unpack2(fma2(pack2(sv[c * 32 + e], sv[c * 32 + e + 1]), sl2_2, neg_m2), x0, x1);
-                            const float e0 = ex2(x0), e1 = ex2(x1);
-                            lacc[(e >> 1) & 3] = add2(lacc[(e >> 1) & 3], pack2(e0, e1));
-                            __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
-                            packed[e / 2] = *reinterpret_cast<uint32_t*>(&h);
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(ex2(x0), ex2(x1));
+                            const uint32_t w = *reinterpret_cast<const uint32_t*>(&h);
+                            packed[e / 2] = w;
+                            // (the sum is of the rounded weights, those that multiply V: a row's weights add up to one, and a row that hangs on few keys
+                            // does not carry their rounding)
+                            lacc[(e >> 1) & 3] = add2(lacc[(e >> 1) & 3], pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
                         }
                         tmem_st16u(lane_base + buf * BK + c * 16, packed);
                     }

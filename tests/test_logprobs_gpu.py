@@ -157,6 +157,12 @@ def test_token_logprobs_twice_captured_and_past_32_bit_offsets():
         kernels.token_logprobs(x, dev_ids, *out)
     graph.replay()
     assert all(torch.equal(p.cpu(), q.cpu()) for p, q in zip(a, out))
+    for n, V, top in ((64, 151936, 20), (300, 32003, 8), (1, 151936, 32)):           # one block a row and clusters, the same bits every time
+        y, first = logits(n, V, n), None
+        for _ in range(60):
+            got = [t.cpu() for t in score(y, tokens(n, 1, V, 2), top)]
+            first = first or got
+            assert all(torch.equal(p, q) for p, q in zip(first, got))
     big = torch.empty(2 ** 31 + 2 ** 20, dtype=torch.bfloat16, device=DEV)
     rows = big.as_strided((2, 30011), (2 ** 31 + 5, 1))
     rows.copy_(x[:2].bfloat16())

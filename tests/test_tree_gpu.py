@@ -228,6 +228,35 @@ def test_attention_tree_behind_32_bit_offsets():
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 64)])
+def test_attention_tree_gives_the_same_bits_every_time(dtype, hd):
+    """Ragged batches whose blocks take pieces of several sequences, two hundred times over under full load of the memory."""
+    g = torch.Generator(DEV).manual_seed(1)
+    contexts, nodes = [4 + 277 * i for i in range(19)], [2 + i * 7 % 13 for i in range(19)]
+    from rocml_b200 import kernels
+    pages = [-(-(c + n) // 64) for c, n in zip(contexts, nodes)]
+    order = torch.randperm(sum(pages), generator=torch.Generator().manual_seed(2)).tolist()
+    table = torch.full((19, max(pages)), -1, dtype=torch.int32)
+    for b, p in enumerate(pages):
+        table[b, :p] = torch.tensor([order.pop() for _ in range(p)])
+    cu = [0]
+    for n in nodes:
+        cu.append(cu[-1] + n)
+    rng = random.Random(3)
+    visible = torch.cat([plain_tree.bits_of(plain_tree.random_parents(rng, n), 1) for n in nodes]).to(DEV)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    k, v = (torch.randn((sum(pages), 8, 64, hd), generator=g, device=DEV).to(dtype) for _ in range(2))
+    q = (torch.randn((cu[-1], 40 * hd), generator=g, device=DEV) * 2).to(dtype)
+    out, first = torch.zeros_like(q), None
+    args = (table.to(DEV), i32(list(range(19))), i32(cu), i32([c + n for c, n in zip(contexts, nodes)]), visible)
+    for _ in range(200):
+        out.zero_()
+        kernels.attention_tree(q, out, k, v, *args, 19, max(nodes), 40, 8, hd, hd ** -0.5, max_kv_len=5200)
+        first = out.clone() if first is None else first
+        assert torch.equal(out, first)
+    kernels.check_status(DEV)
+
+
 # ---- settling a tree ---------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,hd,layers,nkv", [(torch.bfloat16, 128, 3, 2), (torch.float32, 48, 2, 1), (torch.bfloat16, 30, 1, 3), (torch.float32, 3, 2, 2)])
