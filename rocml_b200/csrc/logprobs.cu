@@ -1,18 +1,20 @@
 // Log probabilities of given tokens, the rows' entropy and their most likely tokens, in one pass over the logits.
 //
-// With c >= 0 chosen near the row's maximum, in base 2:   s = sum 2^(x log2 e - c),   t = sum (x log2 e - c) 2^(x log2 e - c),
-//     log sum exp = (c + log2 s) ln 2,   log p(token) = x - log sum exp,   entropy = (log2 s - t / s) ln 2.
-// Each thread carries (c, s, t) of its own elements with c its running maximum; triples are joined pairwise.  Sums are 32-bit, the last
-// line is 64-bit (c may be large beside what is left of it).
+// With m the row's maximum, d = (x - m) log2 e, and n elements that are the maximum:   s = sum of 2^d over the others,   t = sum d 2^d,
+//     log p(token) = (x - m) - log(n + s),   entropy = log(n + s) - t / ((n + s) log2 e).
+// Each thread carries (m, n, s, t) of its own elements with m its running maximum; a warp raises its own to their maximum and adds them up.  Tokens are often nearly certain, and then
+// both results hang on s alone, which a one beside it would swallow: hence n apart, and log1p(s) where n is one.  All sums are 32-bit, a chunk's terms
+// added among themselves first (three hundred small terms, one by one, on top of a sum that already holds a large one would each be rounded at its size).
 //
-// The k most likely, largest first, equal ones by their index.  Beside its triple a thread keeps its largest element (and that
+// The k most likely, largest first, equal ones by their index.  Beside its sums a thread keeps its largest element (and that
 // element's chunk).  All of the k largest elements belong to the k threads whose largest elements lead: any other thread is
 // behind k elements already.  So one pass over the row is enough; afterwards only those k threads' elements (k / threads of the
 // row) are read again, all at once.  Keys are 64-bit whole numbers that order like (value, -index); places are found by counting the keys ahead.
 //
 // A row is read by one block or by the blocks of a cluster, which meet in the first one's shared memory.
 //
-// Memory bounds it where there are rows enough (2,047 rows of 151,936: 190 us, 6.5 TB/s); one row with 20 alternatives takes 7.6 us, 4.5 of them without.
+// Memory bounds it where there are rows enough (2,047 rows of 151,936: 192 us, 6.5 TB/s); one row with 20 alternatives takes 7.8 us, 4.6 of them without.
+// The ones counted apart cost 1 % of 32-bit rows; packed arithmetic and packed maxima give it back, and 5 % more, to bf16 ones, which the arithmetic bounds.
 #include "common.cuh"
 #include "api.h"
 #include "per_device.h"
@@ -20,9 +22,7 @@
 
 namespace {
 constexpr float LOG2E = 1.4426950408889634f;
-// Back from base 2 with the very factor that the logits were multiplied by: a 32-bit log2 e is 2^-25 off, which times a logit of 30 would be seen.
-constexpr double FROM_LOG2 = 1.0 / (double)LOG2E;
-constexpr float NEG_BIG = -1e30f;
+constexpr float LOWEST = -3.402823466e38f;          // (a row may be all of the type's lowest value)
 constexpr int THREADS = 256, WARPS = THREADS / 32, MAX_TOP = 32, MAX_BLOCKS = 16;
 constexpr int UNROLL = 4;          // chunks of 32 bytes that a thread has asked for at once
 typedef unsigned long long Key;
@@ -69,13 +69,48 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return d;
 }
 
-struct Sum { float c, s, t; };
-__device__ __forceinline__ Sum join(Sum a, Sum b) {
-    const float c = fmaxf(a.c, b.c);
-    const float fa = rb::ex2(a.c - c), fb = rb::ex2(b.c - c);
-    // (x log2 e - c) = (x log2 e - a.c) + (a.c - c); an empty side (s = 0) brings nothing
-    const float ta = a.s > 0.f ? fa * fmaf(a.c - c, a.s, a.t) : fa * a.s, tb = b.s > 0.f ? fb * fmaf(b.c - c, b.s, b.t) : fb * b.s;
-    return Sum{c, fmaf(fa, a.s, fb * b.s), ta + tb};
+// Two 32-bit values in one instruction.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void unpair(Pair v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ Pair pair_add(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair pair_mul(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+struct __align__(16) Sum { float m, n, s, t; };
+// The same sums relative to a maximum that is larger.
+__device__ __forceinline__ void raise_maximum(Sum& a, float m) {
+    const float by = max_nan((a.m - m) * LOG2E, -1000.f), f = rb::ex2(by), s = a.n + a.s;
+    a = Sum{m, 0.f, f * s, f * fmaf(by, s, a.t)};
+}
+// A warp's sums joined, in every lane: its maximum first, so that each is raised once and the rest is adding up.
+__device__ __forceinline__ Sum warp_sum(Sum v) {
+    const unsigned int u = __float_as_uint(v.m + 0.f), top = __reduce_max_sync(0xffffffffu, (u & 0x80000000u) ? ~u : u | 0x80000000u);
+    const float m = __uint_as_float((top & 0x80000000u) ? top & 0x7fffffffu : ~top);
+    if (v.m < m) raise_maximum(v, m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v.n += __shfl_xor_sync(0xffffffffu, v.n, o);
+        v.s += __shfl_xor_sync(0xffffffffu, v.s, o);
+        v.t += __shfl_xor_sync(0xffffffffu, v.t, o);
+    }
+    return v;
 }
 
 template <typename T> struct Chunk;                  // 32 bytes
@@ -91,6 +126,27 @@ __device__ __forceinline__ void unpack_chunk(const uint4& a, const uint4& b, flo
     for (int i = 0; i < 8; ++i) {
         if constexpr (Chunk<T>::E == 8) x[i] = __uint_as_float(w[i]);
         else { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+}
+template <int E>
+__device__ __forceinline__ float largest(const float* x) {
+    float mx = x[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) mx = fmaxf(mx, x[e]);
+    return mx;
+}
+// The largest of eight words' values, as they lie in memory.
+template <typename T>
+__device__ __forceinline__ float largest_packed(const uint4& a, const uint4& b) {
+    if constexpr (Chunk<T>::E == 8) {
+        float x[8];
+        unpack_chunk<T>(a, b, x);
+        return largest<8>(x);
+    } else {
+        auto two = [](unsigned int w) { return *reinterpret_cast<__nv_bfloat162*>(&w); };
+        const __nv_bfloat162 m = __hmax2(__hmax2(__hmax2(two(a.x), two(a.y)), __hmax2(two(a.z), two(a.w))),
+                                         __hmax2(__hmax2(two(b.x), two(b.y)), __hmax2(two(b.z), two(b.w))));
+        return fmaxf(__low2float(m), __high2float(m));
     }
 }
 // The chunk whose first element is `i0` (which may lie before the row, or end after it: -inf there).
@@ -134,15 +190,10 @@ __device__ __forceinline__ Key block_merge(Shared& sh, Key v, int lists = WARPS,
     return v;
 }
 
-// `n` triples joined (at most 16), by warp 0.
+// `n` sums joined (at most 16), by warp 0.
 __device__ __forceinline__ void sum_up(Shared& sh, int n) {
     const int lane = threadIdx.x & 31;
-    Sum v = lane < n ? sh.sums[lane] : Sum{NEG_BIG, 0.f, 0.f};
-#pragma unroll
-    for (int o = MAX_BLOCKS / 2; o > 0; o >>= 1) {
-        Sum other{__shfl_xor_sync(0xffffffffu, v.c, o), __shfl_xor_sync(0xffffffffu, v.s, o), __shfl_xor_sync(0xffffffffu, v.t, o)};
-        v = join(v, other);
-    }
+    const Sum v = warp_sum(lane < n ? sh.sums[lane] : Sum{LOWEST, 0.f, 0.f, 0.f});
     if (lane == 0) sh.sum = v;
 }
 
@@ -162,37 +213,33 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const i
     const int n_chunks = (V + before + E - 1) / E;
     const int lo = (int)((long long)n_chunks * part / blocks), hi = (int)((long long)n_chunks * (part + 1) / blocks);
 
-    Sum mine{NEG_BIG, 0.f, 0.f};
+    Sum mine{LOWEST, 0.f, 0.f, 0.f};
     float best = -INFINITY;
     int best_chunk = lo + (int)threadIdx.x < hi ? lo + (int)threadIdx.x : -1;
-    // A chunk's exponentials are added among themselves first: three hundred small terms, one by one, on top of a sum that already holds a large one
-    // would each be rounded at its size.
     auto add_chunk = [&](const float* x) {
-        float s2[2] = {0.f, 0.f}, t2[2] = {0.f, 0.f};
+        float s2[2] = {0.f, 0.f}, n2[2] = {0.f, 0.f}, t2[2];
+        Pair t = 0ull;
+        const Pair less_m = pair(-mine.m, -mine.m), log2e = pair(LOG2E, LOG2E);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float d = max_nan(fmaf(x[e], LOG2E, -mine.c), -1000.f);       // (-inf: 2^-1000 is 0, and so is 0 times -1000)
-            const float p = rb::ex2(d);
-            s2[e & 1] += p;
-            t2[e & 1] = fmaf(d, p, t2[e & 1]);
+        for (int e = 0; e < E; e += 2) {
+            float d[2], p[2];
+            unpair(pair_mul(pair_add(pair(x[e], x[e + 1]), less_m), log2e), d[0], d[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                d[i] = max_nan(d[i], -1000.f);             // (-inf: 2^-1000 is 0, and so is 0 times -1000)
+                p[i] = rb::ex2(d[i]);
+                if (d[i] == 0.f) n2[i] += 1.f;
+                else s2[i] += p[i];
+            }
+            t = pair_fma(pair(d[0], d[1]), pair(p[0], p[1]), t);
         }
+        unpair(t, t2[0], t2[1]);
+        mine.n += n2[0] + n2[1];
         mine.s += s2[0] + s2[1];
         mine.t += t2[0] + t2[1];
     };
-    auto largest = [&](const float* x) {
-        float mx = x[0];
-#pragma unroll
-        for (int e = 1; e < E; ++e) mx = fmaxf(mx, x[e]);
-        return mx;
-    };
     auto new_maximum = [&](float mx) {
-        const float c_new = fmaxf(mine.c, mx * LOG2E);
-        if (c_new > mine.c) {
-            const float f = rb::ex2(mine.c - c_new);
-            mine.t = mine.s > 0.f ? f * fmaf(mine.c - c_new, mine.s, mine.t) : f * mine.s;
-            mine.s *= f;
-            mine.c = c_new;
-        }
+        if (mx > mine.m) raise_maximum(mine, mx);
     };
     // whole chunks, UNROLL of them at a time; the row's first and last chunk, which it may share with its neighbours, one by one
     const int inner_lo = max(lo, before > 0 ? 1 : 0), inner_hi = min(hi, (int)(((long long)V + before) / E));
@@ -200,7 +247,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const i
     if (c < hi && c < inner_lo) {
         float x[E];
         load_chunk(row, c * E - before, V, x);
-        best = largest(x);
+        best = largest<E>(x);
         new_maximum(best);
         add_chunk(x);
         c += THREADS;
@@ -216,9 +263,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const i
         float mx[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            float x[E];
-            unpack_chunk<T>(raw[u][0], raw[u][1], x);
-            mx[u] = largest(x);
+            mx[u] = largest_packed<T>(raw[u][0], raw[u][1]);
             if (c + u * THREADS < inner_hi && mx[u] > best) { best = mx[u]; best_chunk = c + u * THREADS; }
         }
         float all = mx[0];
@@ -235,16 +280,12 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const i
     if (inner_hi < hi && hi - 1 >= inner_lo && (hi - 1 - lo) % THREADS == (int)threadIdx.x) {
         float x[E];
         load_chunk(row, (hi - 1) * E - before, V, x);
-        const float mx = largest(x);
+        const float mx = largest<E>(x);
         if (mx > best) { best = mx; best_chunk = hi - 1; }
         new_maximum(mx);
         add_chunk(x);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Sum other{__shfl_xor_sync(0xffffffffu, mine.c, o), __shfl_xor_sync(0xffffffffu, mine.s, o), __shfl_xor_sync(0xffffffffu, mine.t, o)};
-        mine = join(mine, other);
-    }
+    mine = warp_sum(mine);
     if (lane == 0) sh.sums[warp] = mine;
     __syncthreads();
     if (warp == 0) sum_up(sh, WARPS);
@@ -348,9 +389,8 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const i
                 const int p = warp + i * WARPS;
                 if (p >= blocks) continue;
                 const uint32_t at = sm100::map_to_cta(sm100::smem_u32(&sh.sum), p);
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[i].c) : "r"(at));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[i].s) : "r"(at + 4));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[i].t) : "r"(at + 8));
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(v[i].m), "=f"(v[i].n), "=f"(v[i].s), "=f"(v[i].t) : "r"(at));
                 if (top > 0)
                     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k[i]) : "r"(sm100::map_to_cta(sm100::smem_u32(&sh.best[lane]), p)));
             }
@@ -376,18 +416,18 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const i
         if (part != 0) return;
     }
     const Sum all = sh.sum;
-    const float log_s = log2f(all.s);
-    const double lse = ((double)all.c + (double)log_s) * FROM_LOG2;
-    const bool nothing = all.s == 0.f;                   // every logit -inf: nothing has a probability
-    if (entropy && threadIdx.x == 0) entropy[r] = nothing ? 0.f : (float)((double)(log_s - all.t / all.s) * FROM_LOG2);
+    const float total = all.n + all.s, log_s = all.n == 1.f && all.s < 1.f ? log1pf(all.s) : logf(total);
+    auto logprob = [&](float x) { return (float)(((double)x - (double)all.m) - (double)log_s); };
+    const bool nothing = total == 0.f;                   // every logit -inf: nothing has a probability
+    if (entropy && threadIdx.x == 0) entropy[r] = nothing ? 0.f : (float)((double)log_s - (double)all.t / ((double)total * (double)LOG2E));
     for (int j = threadIdx.x; j < m; j += THREADS) {
         const int id = ids[(size_t)r * m + j];
-        logprobs[(size_t)r * m + j] = id < 0 || id >= V || nothing ? -INFINITY : (float)((double)rb::to_f32(row[id]) - lse);
+        logprobs[(size_t)r * m + j] = id < 0 || id >= V || nothing ? -INFINITY : logprob(rb::to_f32(row[id]));
     }
     if ((int)threadIdx.x < top) {
         const Key k = sh.best[threadIdx.x];
         if (top_ids) top_ids[(size_t)r * top + threadIdx.x] = k ? key_index(k) : -1;
-        if (top_logprobs) top_logprobs[(size_t)r * top + threadIdx.x] = !k || nothing ? -INFINITY : (float)((double)key_value(k) - lse);
+        if (top_logprobs) top_logprobs[(size_t)r * top + threadIdx.x] = !k || nothing ? -INFINITY : logprob(key_value(k));
     }
 }
 }  // namespace

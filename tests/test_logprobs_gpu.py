@@ -167,3 +167,52 @@ def test_token_logprobs_twice_captured_and_past_32_bit_offsets():
     rows = big.as_strided((2, 30011), (2 ** 31 + 5, 1))
     rows.copy_(x[:2].bfloat16())
     check(rows, ids[:2], 8)
+
+
+@pytest.mark.parametrize("V,top", [(2, 1), (33, 4), (9001, 0), (50257, 20), (151936, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gap", [4.0, 14.0, 24.0])
+def test_token_logprobs_of_nearly_certain_tokens_are_relative(V, top, dtype, gap):
+    """What a nearly certain token's probability lacks is the other tokens' share, and that is held to its own size.  A term's exponent d (in base 2, not
+    below -70: what lies lower is less than 2^-20 of the share) is rounded twice and multiplied by a log2 e that is 1.4e-8 off: 70 ln 2 (2^-23 + 1.4e-8) =
+    6.5e-6 of the term.  The special-function unit gives 2^-22 for the term and for each of some 20 raised maxima: 5e-6.  Chunks of 16: 1e-6.  Together
+    1.3e-5, and the results' own roundings."""
+    g = torch.Generator().manual_seed(V + int(gap))
+    x = (torch.randn((6, V), generator=g) * 2).to(dtype)
+    at = torch.tensor([0, V - 1, V // 2, V // 3, min(V - 1, 8), min(V - 1, 1000)])
+    x[torch.arange(6), at] = (x.float().amax(1) + gap).to(dtype)
+    d = x.double() - x.double().amax(1, keepdim=True)
+    others = torch.where(torch.arange(V) == at[:, None], 0.0, d.exp())
+    log_s = torch.log1p(others.sum(1))
+    want = -log_s[:, None], log_s - (others * d).sum(1) / (1 + others.sum(1))
+    for rows in (slice(0, 6), slice(2, 3)):
+        got = score(x.to(DEV)[rows], at[rows, None].int(), top)
+        for a, b in ((got[0], want[0][rows]), (got[1], want[1][rows])):
+            a, b = a.double().cpu(), b.double()
+            assert ((a - b).abs() <= 1.5e-5 * b.abs()).all(), ((a - b).abs() / b.abs()).max().item()
+        if top:
+            assert torch.equal(got[2].cpu()[:, 0], got[0][:, 0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_token_logprobs_of_the_types_lowest_and_highest_values(dtype):
+    V = 4099
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x = torch.full((5, V), low, dtype=dtype)
+    x[1, 7], x[2, [7, 4098]], x[3, 0] = high, 0.0, -math.inf
+    x[4] = torch.randn(V, generator=torch.Generator().manual_seed(1)).to(dtype)
+    x[4, 1::2] = low
+    ids = torch.tensor([[0, V - 1], [7, 8], [7, 4098], [1, 0], [2, 3]], dtype=torch.int32)
+    got = score(x.to(DEV), ids, 2)
+    a = math.log(V)
+    want = torch.tensor([[-a, -a], [0.0, -math.inf], [-math.log(2), -math.log(2)], [-math.log(V - 1), -math.inf]], dtype=torch.float64)
+    lp = got[0].double()
+    for r, c in ((0, 0), (0, 1), (1, 0), (2, 0), (2, 1), (3, 0), (3, 1)):
+        close(lp[r, c].reshape(1), want[r, c].reshape(1), "given")
+    close(got[1][:4], torch.tensor([a, 0.0, math.log(2), math.log(V - 1)], dtype=torch.float64), "entropy")
+    # a difference past the type's range, or just short of it: not above the lowest value
+    assert lp[1, 1] <= low and lp[4, 1] <= 0.99 * low
+    rest = plain_tree.logprobs(x[4:, ::2].contiguous(), torch.tensor([[1]], dtype=torch.int32), 2)
+    close(got[0][4:, :1], rest[0], "given")
+    close(got[1][4:], rest[1], "entropy")
+    assert got[3].tolist()[0] == [0, 1] and got[3].tolist()[2] == [7, 4098]
