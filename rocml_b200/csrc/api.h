@@ -363,13 +363,26 @@ int rb_attention_tree(const RbTreeCall* call, void* stream);
 
 // Which nodes of every tree the sampled tokens confirm (path [n_seqs, path_ld], counts, next_token) and, when k and v ([layers, n_pages, nkv, 64,
 // row_bytes]) are given, the confirmed nodes' keys and values moved to the places behind the context (tree_accept.cu).
-int rb_tree_accept(const int* tokens, const int* parents, const int* visible, int words, const int* sampled, const int* cu_q, int n_seqs,
-                   int* path, int path_ld, int* counts, int* next_token, const int* seq_slot, const int* kv_len, const int* block_table,
-                   int max_pages, void* k, void* v, int layers, int nkv, long long n_pages, int row_bytes, int element_bytes, void* stream);
+typedef struct RbAcceptCall {
+    const int *tokens, *parents, *visible, *sampled, *cu_q;
+    int *path, *counts, *next_token;
+    const int *seq_slot, *kv_len, *block_table;
+    void *k, *v;
+    long long n_pages;
+    int words, n_seqs, path_ld, max_pages, layers, nkv, row_bytes, element_bytes;
+} RbAcceptCall;
+int rb_tree_accept(const RbAcceptCall* call, void* stream);
 
 // Log probabilities of given tokens, entropy and the `top` most likely tokens of rows of logits (logprobs.cu).
-int rb_token_logprobs(const void* logits, int dtype, long long ld, int n, int V, const int* ids, int m, float* logprobs, float* entropy,
-                      float* top_logprobs, int* top_ids, int top, int blocks, void* stream);
+typedef struct RbLogprobsCall {
+    const void* logits;
+    const int* ids;
+    float *logprobs, *entropy, *top_logprobs;
+    int* top_ids;
+    long long ld;
+    int dtype, n, vocab, m, top, blocks;
+} RbLogprobsCall;
+int rb_token_logprobs(const RbLogprobsCall* call, void* stream);
 
 #ifdef __cplusplus
 }

@@ -434,16 +434,17 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const i
 
 // logits [n, V] (row stride ld elements); ids int32 [n, m]; logprobs float32 [n, m]; entropy float32 [n] or null; top_logprobs float32 and
 // top_ids int32 [n, top], top <= 32.  blocks: 1, 2, 4, 8 or 16 blocks a row.
-extern "C" int rb_token_logprobs(const void* logits, int dtype, long long ld, int n, int V, const int* ids, int m, float* logprobs,
-                                 float* entropy, float* top_logprobs, int* top_ids, int top, int blocks, void* stream) {
-    if (n <= 0) return RB_OK;
-    if (V <= 0 || V > (1 << 30) || m < 0 || top < 0 || top > MAX_TOP || top > V || (m > 0 && (!ids || !logprobs)) || blocks < 1 || blocks > 16 ||
-        (blocks & (blocks - 1)) || (long long)n * blocks > 0x7fffffffll)
+extern "C" int rb_token_logprobs(const RbLogprobsCall* call, void* stream) {
+    const RbLogprobsCall& c = *call;
+    if (c.n <= 0) return RB_OK;
+    if (c.vocab <= 0 || c.vocab > (1 << 30) || c.m < 0 || c.top < 0 || c.top > MAX_TOP || c.top > c.vocab || (c.m > 0 && (!c.ids || !c.logprobs)) ||
+        c.blocks < 1 || c.blocks > MAX_BLOCKS || (c.blocks & (c.blocks - 1)) || (long long)c.n * c.blocks > 0x7fffffffll)
         return RB_ERR_BAD_SIZE;
     cudaStream_t st = (cudaStream_t)stream;
     auto go = [&](auto kernel, auto* x, rb::PerDevice<int>& allowed) -> int {
-        if (blocks == 1) {
-            RB_LAUNCH((kernel), dim3(n), dim3(THREADS), 0, st, x, ld, V, ids, m, logprobs, entropy, top_logprobs, top_ids, top, blocks);
+        if (c.blocks == 1) {
+            RB_LAUNCH((kernel), dim3(c.n), dim3(THREADS), 0, st, x, c.ld, c.vocab, c.ids, c.m, c.logprobs, c.entropy, c.top_logprobs, c.top_ids, c.top,
+                      c.blocks);
             return RB_OK;
         }
         int device;
@@ -452,12 +453,14 @@ extern "C" int rb_token_logprobs(const void* logits, int dtype, long long ld, in
         const int* known;
         const int rc = allowed.get(device, &known, [&](int&) { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); });
         if (rc) return rc;
-        e = rb::launch_clustered(kernel, dim3(n * blocks), dim3(THREADS), dim3(blocks), 0, st, x, ld, V, ids, m, logprobs, entropy, top_logprobs,
-                                 top_ids, top, blocks);
+        e = rb::launch_clustered(kernel, dim3(c.n * c.blocks), dim3(THREADS), dim3(c.blocks), 0, st, x, c.ld, c.vocab, c.ids, c.m, c.logprobs, c.entropy,
+                                 c.top_logprobs, c.top_ids, c.top, c.blocks);
         return (int)e;
     };
     static rb::PerDevice<int> allowed_f32, allowed_bf16;
-    if (dtype == RB_F32) return ((uintptr_t)logits & 3) ? RB_ERR_BAD_ALIGN : go(token_logprobs_kernel<float>, (const float*)logits, allowed_f32);
-    if (dtype == RB_BF16) return ((uintptr_t)logits & 1) ? RB_ERR_BAD_ALIGN : go(token_logprobs_kernel<__nv_bfloat16>, (const __nv_bfloat16*)logits, allowed_bf16);
+    if (c.dtype == RB_F32)
+        return ((uintptr_t)c.logits & 3) ? RB_ERR_BAD_ALIGN : go(token_logprobs_kernel<float>, (const float*)c.logits, allowed_f32);
+    if (c.dtype == RB_BF16)
+        return ((uintptr_t)c.logits & 1) ? RB_ERR_BAD_ALIGN : go(token_logprobs_kernel<__nv_bfloat16>, (const __nv_bfloat16*)c.logits, allowed_bf16);
     return RB_ERR_BAD_DTYPE;
 }

@@ -104,36 +104,30 @@ tree_accept_kernel(const int* __restrict__ tokens, const int* __restrict__ paren
 }
 
 template <typename Vec>
-int launch_accept(const int* tokens, const int* parents, const int* visible, int words, const int* sampled, const int* cu_q, int n_seqs,
-                  int* path, int path_ld, int* counts, int* next_token, const int* seq_slot, const int* kv_len, const int* block_table,
-                  int max_pages, void* k, void* v, int layers, int nkv, long long n_pages, int row_bytes, cudaStream_t stream) {
-    const int vecs = row_bytes / (int)sizeof(Vec);
-    const long long threads = k ? (v ? 2ll : 1ll) * layers * nkv * vecs : 1;
+int launch_accept(const RbAcceptCall& c, cudaStream_t stream) {
+    const int vecs = c.row_bytes / (int)sizeof(Vec);
+    const long long threads = c.k ? (c.v ? 2ll : 1ll) * c.layers * c.nkv * vecs : 1;
     const long long blocks = (threads + THREADS - 1) / THREADS;
     // about one wave of blocks over all sequences: each finds the path once, whatever it moves
-    const long long wave = (5 * 148 + n_seqs - 1) / n_seqs;
+    const long long wave = (5 * 148 + c.n_seqs - 1) / c.n_seqs;
     const unsigned x_blocks = (unsigned)(blocks < wave ? blocks : wave);
-    RB_LAUNCH((tree_accept_kernel<Vec>), dim3(x_blocks, n_seqs), dim3(THREADS), 0, stream, tokens, parents, visible, words, sampled, cu_q,
-              path, path_ld, counts, next_token, seq_slot, kv_len, block_table, max_pages, (Vec*)k, (Vec*)v, layers * nkv, nkv, n_pages, vecs);
+    RB_LAUNCH((tree_accept_kernel<Vec>), dim3(x_blocks, c.n_seqs), dim3(THREADS), 0, stream, c.tokens, c.parents, c.visible, c.words, c.sampled, c.cu_q,
+              c.path, c.path_ld, c.counts, c.next_token, c.seq_slot, c.kv_len, c.block_table, c.max_pages, (Vec*)c.k, (Vec*)c.v, c.layers * c.nkv, c.nkv,
+              c.n_pages, vecs);
     return RB_OK;
 }
 }  // namespace
 
 // k, v: [layers, n_pages, nkv, 64, row_bytes]; v null: one tensor serves as both; both null: nothing is moved.
-extern "C" int rb_tree_accept(const int* tokens, const int* parents, const int* visible, int words, const int* sampled, const int* cu_q,
-                              int n_seqs, int* path, int path_ld, int* counts, int* next_token, const int* seq_slot, const int* kv_len,
-                              const int* block_table, int max_pages, void* k, void* v, int layers, int nkv, long long n_pages,
-                              int row_bytes, int element_bytes, void* stream) {
-    if (n_seqs <= 0) return RB_OK;
-    if (words <= 0 || words > WORDS || path_ld <= 0 || path_ld > MAX_NODES || n_seqs > 65535) return RB_ERR_BAD_SIZE;
-    if ((v && !k) || (k && k == v)) return RB_ERR_BAD_SIZE;          // (one tensor for both is moved once)
-    if (k && (!seq_slot || !kv_len || !block_table || layers <= 0 || nkv <= 0 || row_bytes <= 0 || max_pages <= 0)) return RB_ERR_BAD_SIZE;
+extern "C" int rb_tree_accept(const RbAcceptCall* call, void* stream) {
+    const RbAcceptCall& c = *call;
+    if (c.n_seqs <= 0) return RB_OK;
+    if (c.words <= 0 || c.words > WORDS || c.path_ld <= 0 || c.path_ld > MAX_NODES || c.n_seqs > 65535) return RB_ERR_BAD_SIZE;
+    if ((c.v && !c.k) || (c.k && c.k == c.v)) return RB_ERR_BAD_SIZE;          // (one tensor for both is moved once)
+    if (c.k && (!c.seq_slot || !c.kv_len || !c.block_table || c.layers <= 0 || c.nkv <= 0 || c.row_bytes <= 0 || c.max_pages <= 0)) return RB_ERR_BAD_SIZE;
     cudaStream_t st = (cudaStream_t)stream;
-#define RB_ACCEPT_ARGS tokens, parents, visible, words, sampled, cu_q, n_seqs, path, path_ld, counts, next_token, seq_slot, kv_len, block_table, \
-                       max_pages, k, v, layers, nkv, n_pages, row_bytes, st
-    if (!k || (row_bytes % 16 == 0 && !(((uintptr_t)k | (uintptr_t)v) & 15))) return launch_accept<uint4>(RB_ACCEPT_ARGS);
-    if (element_bytes == 4 && row_bytes % 4 == 0) return launch_accept<uint32_t>(RB_ACCEPT_ARGS);
-    if (element_bytes == 2 && row_bytes % 2 == 0) return launch_accept<uint16_t>(RB_ACCEPT_ARGS);
+    if (!c.k || (c.row_bytes % 16 == 0 && !(((uintptr_t)c.k | (uintptr_t)c.v) & 15))) return launch_accept<uint4>(c, st);
+    if (c.element_bytes == 4 && c.row_bytes % 4 == 0) return launch_accept<uint32_t>(c, st);
+    if (c.element_bytes == 2 && c.row_bytes % 2 == 0) return launch_accept<uint16_t>(c, st);
     return RB_ERR_BAD_DTYPE;
-#undef RB_ACCEPT_ARGS
 }

@@ -182,7 +182,6 @@ class TreeSteps:
 
     def _verify_piece(self, entries, params, rngs, histories):
         eng = self.engine
-        kept = {}
         try:
             logits, buf, depths = self._run(entries)
             if self._sampler is None:
@@ -221,7 +220,6 @@ class TreeSteps:
             results = []
             for e, p, r, way, count, last in zip(entries, params, rngs, paths, counts, nxt):
                 eng.cache.commit(e.slot, count)
-                kept[e.slot] = True
                 if not p.is_greedy:
                     for _ in range(count):
                         r.next_f32()

@@ -223,8 +223,8 @@ def _lib():
                                              _vp, _i, _vp]
         lib.rb_low_rank.argtypes = [_vp, _i, _i, _ll, _i, _i, _i, _vp, _i, _i, _i, _vp, _i, _i, _i, _vp, _i, _vp]
         lib.rb_attention_tree.argtypes = [_c.c_char_p, _vp]
-        lib.rb_tree_accept.argtypes = [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _ll, _i, _i, _vp]
-        lib.rb_token_logprobs.argtypes = [_vp, _i, _ll, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _vp]
+        lib.rb_tree_accept.argtypes = [_c.c_char_p, _vp]
+        lib.rb_token_logprobs.argtypes = [_c.c_char_p, _vp]
         lib.rb_gemm_tcgen05_set_wait.argtypes = [_ll, _i]
         lib.rb_gemm_tcgen05_set_wait.restype = None
         _sigs_done = True
@@ -926,8 +926,14 @@ def _tree_sizes(what: str, visible, cu_q, n_seqs: int, max_nodes: int):
     return tokens, words
 
 
-# RbTreeCall of csrc/api.h (one packed argument: converting thirty costs microseconds)
-_TREE_CALL = struct.Struct("@13P2q14i3f")
+# RbTreeCall, RbAcceptCall and RbLogprobsCall of csrc/api.h (one packed argument: converting thirty costs microseconds)
+_TREE_CALL = struct.Struct("@13P2q14i3f4x")
+_ACCEPT_CALL = struct.Struct("@13Pq8i")
+_LOGPROBS_CALL = struct.Struct("@6Pq6i")
+
+
+def _or_null(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def tree_shares(pairs: int, units: int, rows: int, nkv: int, slots: int) -> int:
@@ -1001,7 +1007,7 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     work = torch.empty(words_of_work, dtype=torch.float32, device=device) if words_of_work else None
     call = _TREE_CALL.pack(
         *pointers, block_table.data_ptr(), seq_slot.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
-        0 if positions is None else positions.data_ptr(), sinks or 0, 0 if work is None else work.data_ptr(), status_word(device).data_ptr(),
+        _or_null(positions), sinks or 0, _or_null(work), status_word(device).data_ptr(),
         q_stride, o_stride, tokens, dtype_code(dtype), k_cache.shape[0], max_pages, words, n_seqs, max_nodes, nq, nkv, hd, int(window), int(keep),
         shares, rows_tile, scale, one_sink, softcap)
     _check(_lib().rb_attention_tree(call, _stream()), "attention_tree")
@@ -1045,17 +1051,17 @@ def tree_accept(token_ids: torch.Tensor, parents: torch.Tensor, visible: torch.T
                () if k is None else (k, v))
     if n_seqs == 0:
         return
-    pointer = lambda t: None if t is None else t.data_ptr()
-    rc = _lib().rb_tree_accept(
-        token_ids.data_ptr(), parents.data_ptr(), visible.data_ptr(), words, sampled.data_ptr(), cu_q.data_ptr(), n_seqs, path.data_ptr(), path.shape[1],
-        counts.data_ptr(), next_token.data_ptr(), pointer(seq_slot), pointer(kv_len), pointer(block_table), max_pages, pointer(k), pointer(v),
-        layers, nkv, n_pages, row_bytes, esz, _stream())
-    _check(rc, "tree_accept")
+    call = _ACCEPT_CALL.pack(
+        token_ids.data_ptr(), parents.data_ptr(), visible.data_ptr(), sampled.data_ptr(), cu_q.data_ptr(), path.data_ptr(), counts.data_ptr(),
+        next_token.data_ptr(), _or_null(seq_slot), _or_null(kv_len), _or_null(block_table), _or_null(k), _or_null(v), n_pages, words, n_seqs,
+        path.shape[1], max_pages, layers, nkv, row_bytes, esz)
+    _check(_lib().rb_tree_accept(call, _stream()), "tree_accept")
 
 
 LOGPROBS_MAX_TOP = 32
 
 
+@functools.lru_cache(maxsize=4096)
 def logprob_blocks(rows: int, vocab: int, device=0) -> int:
     """Blocks a row of token_logprobs: a power of two that about fills the device once, none with less than 2,048 logits; up to eight, which any
     cluster may have, and sixteen for a few rows only (151,936 logits, 20 alternatives: one row 7.6 us with sixteen, 8.1 with eight, 32 rows 18 and
@@ -1098,11 +1104,9 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor], logprobs: 
     if n == 0:
         return
     _ints_here("token_logprobs", (ids, top_ids), (logits, logprobs, entropy, top_logprobs))
-    pointer = lambda t: None if t is None else t.data_ptr()
-    rc = _lib().rb_token_logprobs(
-        logits.data_ptr(), dtype_code(logits.dtype), logits.stride(0), n, V, pointer(ids), m, pointer(logprobs), pointer(entropy),
-        pointer(top_logprobs), pointer(top_ids), top, logprob_blocks(n, V, logits.device), _stream())
-    _check(rc, "token_logprobs")
+    call = _LOGPROBS_CALL.pack(logits.data_ptr(), _or_null(ids), _or_null(logprobs), _or_null(entropy), _or_null(top_logprobs), _or_null(top_ids),
+                               logits.stride(0), dtype_code(logits.dtype), n, V, m, top, logprob_blocks(n, V, logits.device))
+    _check(_lib().rb_token_logprobs(call, _stream()), "token_logprobs")
 
 
 # ---- tensor-core matrix product (tcgen05) ----------------------------------------------------------------
