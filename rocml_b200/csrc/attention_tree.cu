@@ -16,6 +16,9 @@
 // one that is cut, each share leaves (maximum, sum, unnormalised result) in the work space and attention_tree_merge_kernel joins them.  A
 // share is cut at most at its two ends, so its work space has two places: 2 c for what began earlier, 2 c + 1 for what goes on later.
 //
+// Clusters.  Where a sequence's tile of rows has few pages a block, the blocks of a cluster share them instead and join through each other's shared
+// memory: no second kernel, no way through memory (tensor-core kernel only; kernels.py has the rule and what it was measured with).
+//
 // This file: the entry point, the kernel that joins pieces, and attention_tree_simple_kernel, which takes any head size up to 512 and both types
 // with 32-bit multiply-adds.  attention_tree_tc5.cu: bfloat16 heads of 64, 128 and 256 on the tensor cores.
 #include "api.h"
@@ -89,7 +92,7 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
     int* tl = pre + a.B + 1;
     const int kvh = blockIdx.y;
     const int extra = prefix_tiles(a, pre, tl);
-    Pieces pieces(pre, a.B, a.shares, blockIdx.x, extra);
+    Pieces<false> pieces(a, pre, blockIdx.x, extra);
     if (a.n_notes) note_nothing(a, pieces, pre, tl, kvh, blockIdx.x, threadIdx.x, 128);
     const int rg = threadIdx.x >> 4, kg = threadIdx.x & 15;
     const float sl2 = a.scale * LOG2E;
@@ -477,7 +480,7 @@ extern "C" int rb_attention_tree(const RbTreeCall* call, void* stream) {
     if (x.n_seqs <= 0 || x.max_nodes <= 0) return RB_OK;
     if (x.n_seqs > MAX_SEQS || x.nkv <= 0 || x.nq <= 0 || x.nq % x.nkv || x.hd <= 0 || x.hd > 512 || x.words <= 0 || x.max_nodes > 32 * x.words ||
         x.shares <= 0 || x.shares > 32767 || x.window < 0 || x.keep < 0 || !(x.scale > 0.f) || x.max_pages <= 0 || (x.window > 0 && !x.positions) ||
-        (x.shares > 1 && !x.work) || x.nkv > 65535 || x.rows_tile <= 0)
+        (x.shares > 1 && x.cluster <= 1 && !x.work) || x.nkv > 65535 || x.rows_tile <= 0)
         return RB_ERR_BAD_SIZE;
     if (x.dtype != RB_F32 && x.dtype != RB_BF16) return RB_ERR_BAD_DTYPE;
     if ((uintptr_t)x.work & 15) return RB_ERR_BAD_ALIGN;
@@ -493,7 +496,10 @@ extern "C" int rb_attention_tree(const RbTreeCall* call, void* stream) {
     const long long units = ((long long)x.max_nodes * group + x.rows_tile - 1) / x.rows_tile;
     if (units > 0x7fffffff / MAX_SEQS) return RB_ERR_BAD_SIZE;
     a.max_units = (int)units;
-    if (x.shares > 1) {
+    const bool clustered = x.cluster > 1;
+    if (clustered && (!tc5 || x.cluster > 16 || (x.cluster & (x.cluster - 1)) || x.n_seqs * units * x.cluster > 0x7fffffff)) return RB_ERR_BAD_SIZE;
+    a.cluster = x.cluster;
+    if (x.shares > 1 && !clustered) {
         const size_t places = 2ull * x.shares * x.nkv * x.rows_tile;
         a.part_o = x.work;
         a.part_ml = x.work + places * x.hd;
@@ -511,7 +517,7 @@ extern "C" int rb_attention_tree(const RbTreeCall* call, void* stream) {
         rc = x.dtype == RB_F32 ? launch_any<float>(x.q, x.q_stride, x.out, x.o_stride, x.k_cache, x.v_cache, a, st)
                                : launch_any<__nv_bfloat16>(x.q, x.q_stride, x.out, x.o_stride, x.k_cache, x.v_cache, a, st);
     }
-    if (rc != RB_OK || x.shares == 1) return rc;
+    if (rc != RB_OK || x.shares == 1 || clustered) return rc;
     if (tc5) {
         RB_LAUNCH((attention_tree_merge_rows_kernel), dim3((x.rows_tile + 31) / 32 * (x.hd / (a.notes_by_unit ? JOIN_DIMS : 64)), x.nkv, a.n_notes), dim3(32 * JOIN_WARPS), 0, st, (__nv_bfloat16*)x.out, x.o_stride, a);
         return RB_OK;

@@ -11,6 +11,11 @@
 // Measured: 100,003 keys on 8 heads, 64 rows, 66 us = 6.2 TB/s; 32 sequences of up to 12,100 keys and trees of 9 to 33 nodes, 4 query heads a
 // key/value head, 133 us for 815 MB; a block alone on its multiprocessor 0.95 us a tile, waiting for the ring of two pages.
 //
+// In a cluster (CLUSTER) a block has one piece and leaves its (maximum, sum, unnormalised result) where Q and the rings were; each block then joins a
+// part of the dimensions of all rows, reading its peers' shared memory (a batch of eight parts at a time, none twice: peers that read one block's part
+// again for what is not there took 50 us).  How much is read grows with the rows, so large tiles are joined by the second kernel.  One sequence of 709
+// keys, 16 rows: 10 us, 12 with two kernels, and 5 us less of the host's time.
+//
 // A share may hold pieces of several sequences, one after the other: the rings and the two score buffers run on, Q and O are handed over at
 // the pieces' ends (q_empty, o_free).  P is rounded to bfloat16 for its product, and the row's sum is that of the rounded weights;
 // everything else is 32-bit until the result.
@@ -81,7 +86,58 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, co
     return true;
 }
 
-template <int HD, bool CAP>
+// What the blocks of a cluster found for a tile of rows, joined: each takes a part of the dimensions, of all rows; a thread four dimensions of a row.
+template <int HD>
+__device__ __forceinline__ void join_cluster(const TreeArgs& a, const ClusterShare& share, int kvh, uint32_t part_o, uint32_t part_ml,
+                                             __nv_bfloat16* __restrict__ out, long long o_stride) {
+    constexpr int BATCH = 8;
+    static_assert(HD * BM * 4 <= 2 * Sizes<HD>::STAGES * Sizes<HD>::KV_TILE, "a block's part lies where its rings were");
+    const Seq s = seq_of(a, share.b);
+    const int row0 = share.mt * a.rows_tile, rows = min(a.rows_tile, s.n * a.group - row0);
+    const int d0 = HD / 4 * share.rank / a.cluster, d1 = HD / 4 * (share.rank + 1) / a.cluster;
+    for (int i = threadIdx.x; i < (d1 - d0) * rows; i += blockDim.x) {
+        const int d = d0 + i / rows, r = i - i / rows * rows;
+        const int node = (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
+        const float sink = (a.sinks ? a.sinks[head] : a.sink) * LOG2E;
+        float top = rb::has_sink(sink) ? sink : NEG_BIG, total = rb::has_sink(sink) ? 1.f : 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c0 = 0; c0 < share.parts; c0 += BATCH) {
+            float m[BATCH], l[BATCH], x[BATCH][4];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                m[j] = NEG_BIG;
+                if (c0 + j >= share.parts) continue;
+                const int c = c0 + j;
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m[j]), "=f"(l[j]) : "r"(map_to_cta(part_ml, c) + r * 8));
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[j][0]), "=f"(x[j][1]), "=f"(x[j][2]), "=f"(x[j][3])
+                             : "r"(map_to_cta(part_o, c) + (d * BM + r) * 16));
+            }
+            float top_new = top;
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) top_new = fmaxf(top_new, m[j]);
+            const float old = exp2f(top - top_new);
+            top = top_new;
+            total *= old;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] *= old;
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                const float w = c0 + j < share.parts ? exp2f(m[j] - top) : 0.f;
+                if (w == 0.f) continue;                      // (past the last part, or nothing beside the others)
+                total = fmaf(l[j], w, total);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] = fmaf(x[j][e], w, acc[e]);
+            }
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        uint2 y;
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv), hi = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+        y.x = *reinterpret_cast<const uint32_t*>(&lo);
+        y.y = *reinterpret_cast<const uint32_t*>(&hi);
+        *reinterpret_cast<uint2*>(out + (size_t)(s.q0 + node) * o_stride + (size_t)head * HD + 4 * d) = y;
+    }
+}
+
+template <int HD, bool CAP, bool CLUSTER>
 __global__ void __launch_bounds__(192, Sizes<HD>::BLOCKS_PER_SM)
 attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                           const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ out, long long o_stride, const TreeArgs a,
@@ -122,13 +178,15 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tmem_relinquish();
     }
     tc_fence_before();
-    const int extra = prefix_tiles(a, pre, tl);              // (ends with a block-wide barrier)
+    int extra = 0;
+    if (CLUSTER) __syncthreads();
+    else extra = prefix_tiles(a, pre, tl);                   // (ends with a block-wide barrier)
     tc_fence_after();
     // Only now may later kernels be scheduled: products take their tensor memory before they wait for this kernel, and one that took a
     // multiprocessor's columns ahead of a block of this grid would wait for it for good.
     rb::pdl_trigger();
     const uint32_t tmem_base = bar->tmem_slot;
-    Pieces pieces(pre, a.B, a.shares, blockIdx.x, extra);
+    Pieces<CLUSTER> pieces(a, pre, blockIdx.x, extra);
     int b, mt, p0, p1;
 
     if (warp == 0) {
@@ -252,11 +310,13 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         const rb::SoftCap capped = rb::soft_cap(a.scale, a.softcap);
         bool alive = true;
         int it = 0, piece = 0, checks = 0;      // tiles, pieces and masked tiles so far
-        if (a.n_notes) note_nothing(a, pieces, pre, tl, kvh, blockIdx.x, tid, 128);
+        if constexpr (!CLUSTER)
+            if (a.n_notes) note_nothing(a, pieces, pre, tl, kvh, blockIdx.x, tid, 128);
         while (alive && pieces.next(pre, tl, b, mt, p0, p1)) {
             const Seq s = seq_of(a, b);
             const int row0 = mt * a.rows_tile, rows = min(a.rows_tile, s.n * a.group - row0);
-            if (a.n_notes && tid == 0) note_piece(a, pieces, s, kvh, blockIdx.x, b, mt, p0, p1);
+            if constexpr (!CLUSTER)
+                if (a.n_notes && tid == 0) note_piece(a, pieces, s, kvh, blockIdx.x, b, mt, p0, p1);
             const bool row_here = r < rows, warp_here = quarter * 32 < rows;
             const int node = (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
             float m_used = NEG_BIG, l_sum = 0.f;
@@ -395,8 +455,11 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                 // (a place's result is [HD / 4][rows][4]: a warp writes 32 rows' 16 bytes side by side)
                 const size_t place = (size_t)(2 * blockIdx.x + (p0 == 0 ? 1 : 0)) * a.nkv + kvh;
                 __nv_bfloat16* orow = out + (size_t)(s.q0 + node) * o_stride + (size_t)head * HD;
-                float* prow = a.part_o + place * HD * a.rows_tile + r * 4;
-                if (!whole && row_here) *reinterpret_cast<float2*>(a.part_ml + (place * a.rows_tile + r) * 2) = make_float2(m_used, l_sum);
+                // In a cluster it stays in shared memory: the rings' and Q's last reads are done, and no copy is in flight.
+                const int part_rows = CLUSTER ? BM : a.rows_tile;
+                float* prow = CLUSTER ? reinterpret_cast<float*>(Ks) + r * 4 : a.part_o + place * HD * a.rows_tile + r * 4;
+                float* pml = CLUSTER ? reinterpret_cast<float*>(Qs) + r * 2 : a.part_ml + (place * a.rows_tile + r) * 2;
+                if (!whole && row_here) *reinterpret_cast<float2*>(pml) = make_float2(m_used, l_sum);
 #pragma unroll 1
                 for (int c = 0; c < HD / 64; ++c) {
                     float ov[64];
@@ -415,7 +478,7 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) rb::store4(prow + (size_t)(c * 16 + i) * a.rows_tile * 4, ov + 4 * i);
+                        for (int i = 0; i < 16; ++i) rb::store4(prow + (size_t)(c * 16 + i) * part_rows * 4, ov + 4 * i);
                     }
                 }
             }
@@ -431,6 +494,16 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tc_fence_after();
         tmem_dealloc(tmem_base, Z::TMEM_COLS);
     }
+    if (CLUSTER) {
+        __syncwarp();
+        const ClusterShare share(a, blockIdx.x);
+        if (share.parts < 2) return;                         // (every block of the cluster agrees)
+        cluster_arrive();
+        cluster_wait();
+        join_cluster<HD>(a, share, kvh, smem_u32(Ks), smem_u32(Qs), out, o_stride);
+        cluster_arrive();                                    // (a block stays until its shared memory has been read)
+        cluster_wait();
+    }
 }
 
 int encode(CUtensorMap* map, const void* ptr, int dims, const cuuint64_t* size, const cuuint64_t* strides, const cuuint32_t* box) {
@@ -442,7 +515,7 @@ int encode(CUtensorMap* map, const void* ptr, int dims, const cuuint64_t* size, 
                ? RB_OK : RB_ERR_BAD_SIZE;
 }
 
-template <int HD, bool CAP>
+template <int HD, bool CAP, bool CLUSTER>
 int launch(const void* q, long long q_stride, int T, void* out, long long o_stride, const void* k, const void* v, int n_pages,
            const TreeArgs& a, int* status, cudaStream_t stream) {
     CUtensorMap mq, mk, mv;
@@ -454,14 +527,20 @@ int launch(const void* q, long long q_stride, int T, void* out, long long o_stri
     if ((rc = encode(&mq, q, 3, q_size, q_strides, q_box)) != RB_OK || (rc = encode(&mk, k, 2, c_size, c_strides, c_box)) != RB_OK ||
         (rc = encode(&mv, v, 2, c_size, c_strides, c_box)) != RB_OK)
         return rc;
-    auto kernel = attention_tree_tc5_kernel<HD, CAP>;
+    auto kernel = attention_tree_tc5_kernel<HD, CAP, CLUSTER>;
     static rb::PerDevice<int> allowed;
     int device;
     const cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return (int)e;
     const int* known;
-    rc = allowed.get(device, &known, [&](int&) { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sizes<HD>::SMEM_BYTES); });
+    rc = allowed.get(device, &known, [&](int&) {
+        const int bad = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sizes<HD>::SMEM_BYTES);
+        return bad || !CLUSTER ? bad : (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    });
     if (rc) return rc;
+    if (CLUSTER)
+        return (int)rb::launch_clustered(kernel, dim3(a.B * a.max_units * a.cluster, a.nkv), dim3(192), dim3(a.cluster), Sizes<HD>::SMEM_BYTES, stream, mq,
+                                         mk, mv, (__nv_bfloat16*)out, o_stride, a, status);
     RB_LAUNCH((kernel), dim3(a.shares, a.nkv), dim3(192), Sizes<HD>::SMEM_BYTES, stream, mq, mk, mv, (__nv_bfloat16*)out, o_stride, a, status);
     return RB_OK;
 }
@@ -473,9 +552,16 @@ int launch_tc5(const void* q, long long q_stride, int T, void* out, long long o_
     if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) || q_stride % 8 || o_stride % 8) return RB_ERR_BAD_ALIGN;
     if (T <= 0 || n_pages <= 0 || !status || (long long)n_pages * a.nkv * PAGE > 0x7fffffffll) return RB_ERR_BAD_SIZE;
 #define RB_TREE_ARGS q, q_stride, T, out, o_stride, k, v, n_pages, a, status, stream
-    if (a.softcap > 0.f)
-        return a.hd == 64 ? launch<64, true>(RB_TREE_ARGS) : a.hd == 128 ? launch<128, true>(RB_TREE_ARGS) : launch<256, true>(RB_TREE_ARGS);
-    return a.hd == 64 ? launch<64, false>(RB_TREE_ARGS) : a.hd == 128 ? launch<128, false>(RB_TREE_ARGS) : launch<256, false>(RB_TREE_ARGS);
+#define RB_TREE_HD(HD) \
+    if (a.hd == HD) { \
+        if (a.cluster > 1) return a.softcap > 0.f ? launch<HD, true, true>(RB_TREE_ARGS) : launch<HD, false, true>(RB_TREE_ARGS); \
+        return a.softcap > 0.f ? launch<HD, true, false>(RB_TREE_ARGS) : launch<HD, false, false>(RB_TREE_ARGS); \
+    }
+    RB_TREE_HD(64)
+    RB_TREE_HD(128)
+    RB_TREE_HD(256)
+    return RB_ERR_BAD_SIZE;
+#undef RB_TREE_HD
 #undef RB_TREE_ARGS
 }
 }  // namespace rb_tree

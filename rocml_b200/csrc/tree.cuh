@@ -18,6 +18,7 @@ struct TreeArgs {
     float scale; int window, keep; float sink; const float* sinks; float softcap;
     int shares, rows_tile;           // rows_tile: rows of a tile that are used, a whole number of nodes for the tensor-core kernel
     int max_nodes, max_units;        // nodes and tiles of rows of the largest tree
+    int cluster;                     // > 1: a (sequence, tile of rows) is shared by the blocks of a cluster, which join what they found themselves
     int4* notes; int n_notes, notes_by_unit;      // see note_of
     float* part_o; float* part_ml;   // [2 shares][nkv][rows_tile][hd], [..][2]
 };
@@ -96,17 +97,35 @@ __device__ __forceinline__ int sequence_of(const int* pre, int B, int f) {
     return lo;
 }
 
+// How the blocks of a cluster share a (sequence, tile of rows): `per` tiles of keys each, the last of `parts` blocks what is left, others nothing.
+struct ClusterShare {
+    int b, mt, rank, tiles, per, parts;
+    __device__ ClusterShare(const TreeArgs& a, int block) {
+        const int unit = block / a.cluster;
+        rank = block - unit * a.cluster;
+        b = unit / a.max_units;
+        mt = unit - b * a.max_units;
+        const Seq s = seq_of(a, b);
+        tiles = mt < s.units ? s.tiles : 0;
+        per = max(1, (tiles + a.cluster - 1) / a.cluster);
+        parts = (tiles + per - 1) / per;
+    }
+};
+
 // Walks the pieces that one share holds: of a sequence's tiles of rows one after the other, each over all its tiles of keys.
-struct Pieces {
+template <bool CLUSTER>
+struct Pieces;
+template <>
+struct Pieces<false> {
     int f, end, b, W, shares, extra, begin;      // begin: where the last piece's (sequence, tile of rows) begins
-    __device__ Pieces(const int* pre, int B, int n_shares, int c, int more) : extra(more) {
-        W = pre[B];
-        shares = max(1, min(n_shares, W));           // (no share between two others is empty: joining counts on it)
+    __device__ Pieces(const TreeArgs& a, const int* pre, int c, int more) : extra(more) {
+        W = pre[a.B];
+        shares = max(1, min(a.shares, W));           // (no share between two others is empty: joining counts on it)
         // (64-bit divisions take half a microsecond)
         const bool small = W < 0x7fffffff / (shares + 1);
         f = c >= shares ? 0 : small ? c * W / shares : (int)((long long)c * W / shares);
         end = c >= shares ? 0 : small ? (c + 1) * W / shares : (int)((c + 1ll) * W / shares);
-        b = sequence_of(pre, B, f);
+        b = sequence_of(pre, a.B, f);
     }
     // the next piece: tiles of keys [p0, p1) for tile of rows mt of sequence `seq`; false: none is left
     __device__ bool next(const int* pre, const int* tl, int& seq, int& mt, int& p0, int& p1) {
@@ -128,12 +147,32 @@ struct Pieces {
     // the share that holds pair g: the last c with c W / shares <= g
     __device__ int share_of(int g) const { return (int)(((g + 1ll) * shares - 1) / W); }
 };
+// A cluster's block has one piece at most.
+template <>
+struct Pieces<true> {
+    int b, mt, f, end;
+    __device__ Pieces(const TreeArgs& a, const int*, int block, int) {
+        const ClusterShare c(a, block);
+        b = c.b;
+        mt = c.mt;
+        f = c.rank < c.parts ? c.rank * c.per : 0;
+        end = c.rank < c.parts ? min(f + c.per, c.tiles) : 0;
+    }
+    __device__ bool next(const int*, const int*, int& seq, int& tile_of_rows, int& p0, int& p1) {
+        if (f >= end) return false;
+        seq = b;
+        tile_of_rows = mt;
+        p0 = f;
+        p1 = f = end;
+        return true;
+    }
+};
 
 // What the joining kernel is told, one entry a (sequence, tile of rows) where those are fewer than the shares, else one a share (for what begins in it
 // and goes on in the next): {first token, first row, rows, first share << 16 | last share}; equal shares: nothing to join.
 __device__ __forceinline__ int4* note_of(const TreeArgs& a, int kvh, int entry) { return a.notes + (size_t)kvh * a.n_notes + entry; }
 // One thread of a block calls this for every piece.
-__device__ __forceinline__ void note_piece(const TreeArgs& a, const Pieces& p, const Seq& s, int kvh, int c, int b, int mt, int p0, int p1) {
+__device__ __forceinline__ void note_piece(const TreeArgs& a, const Pieces<false>& p, const Seq& s, int kvh, int c, int b, int mt, int p0, int p1) {
     if (p0 != 0) return;
     const int last = p1 == s.tiles ? c : p.share_of(p.begin + s.tiles - 1);
     const int row0 = mt * a.rows_tile;
@@ -142,7 +181,7 @@ __device__ __forceinline__ void note_piece(const TreeArgs& a, const Pieces& p, c
     else if (last != c) *note_of(a, kvh, c) = note;
 }
 // Every thread of a block calls this once: entries that no piece will fill.
-__device__ __forceinline__ void note_nothing(const TreeArgs& a, const Pieces& p, const int* pre, const int* tl, int kvh, int c, int tid, int threads) {
+__device__ __forceinline__ void note_nothing(const TreeArgs& a, const Pieces<false>& p, const int* pre, const int* tl, int kvh, int c, int tid, int threads) {
     const int4 none = make_int4(0, 0, 0, 0);
     if (a.notes_by_unit) {
         if (c == 0)

@@ -128,7 +128,7 @@ class TreeSteps:
         if prof is None and eng.use_graphs and T <= eng._prompt_graph_tokens:
             from .engine import _bucket
             t_pad, b_pad = _bucket(T, 16), _bucket(B)
-            pads = (t_pad, b_pad, t_pad, min(MAX_NODES, _bucket(max(q_lens), 16)), _bucket(max(kv_len), 4096), False)
+            pads = (t_pad, b_pad, t_pad, min(MAX_NODES, _bucket(max(q_lens), 16)), _bucket(max(kv_len), 1024), False)
             logits = eng._run_graph(eng._tree_graphs, eng.max_graphs, pads, packed, host, T, pads, tree=tree)
             return logits, eng._last_buffers, depths
         from .engine import _bucket

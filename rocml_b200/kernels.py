@@ -927,7 +927,7 @@ def _tree_sizes(what: str, visible, cu_q, n_seqs: int, max_nodes: int):
 
 
 # RbTreeCall, RbAcceptCall and RbLogprobsCall of csrc/api.h (one packed argument: converting thirty costs microseconds)
-_TREE_CALL = struct.Struct("@13P2q14i3f4x")
+_TREE_CALL = struct.Struct("@13P2q15i3f")
 _ACCEPT_CALL = struct.Struct("@13Pq8i")
 _LOGPROBS_CALL = struct.Struct("@6Pq6i")
 
@@ -948,9 +948,22 @@ def tree_shares(pairs: int, units: int, rows: int, nkv: int, slots: int) -> int:
     return max(1, min(slots // nkv if nkv <= slots else -(-4 * slots // nkv), pairs, max(units, pairs // max(1, rows // 16))))
 
 
+def tree_cluster(n_pages: int, units: int, rows: int, nkv: int, slots: int) -> int:
+    """How many blocks of a cluster share a (sequence, tile of rows) and join what they found through each other's shared memory; 0: all heads' work is
+    shared equally (``tree_shares``) and a second kernel joins.  The cluster saves that kernel and the way through memory but has few blocks, and every
+    sequence costs what the longest does: it is taken while a block has few pages (8 heads, one sequence; us here and with two kernels: 4 rows, 300 keys
+    8.5 and 10.6, 3,000 keys 10.5 and 15.3; 64 rows, 1,000 keys 11.4 and 13.5, 6,000 keys 19.2 and 16.8; 128 rows, 1,000 keys 13.7 and 19.4; 8 sequences of
+    64 rows and 1,000 keys 15.4 and 19.2).  Sixteen blocks, which not every part of the device has beside others, only where half a device is enough and
+    rows are few (32 rows, 6,000 keys 14.4, with eight blocks 17.4; 128 rows, 1,000 keys 16.2 and 13.7)."""
+    blocks = 16 if rows <= 32 and n_pages > 16 and 32 * units * nkv <= slots else 8
+    while blocks > 1 and (units * nkv * blocks > slots or blocks // 2 >= n_pages):
+        blocks //= 2
+    return blocks if blocks > 1 and n_pages <= blocks * (5 if rows > 32 else 9) else 0
+
+
 @functools.lru_cache(maxsize=4096)
 def _tree_plan(tensor_cores: bool, n_seqs: int, max_nodes: int, group: int, nkv: int, hd: int, n_pages: int, device: int):
-    """(rows of a tile, blocks that share a head's work, 32-bit words of work space) of a call of attention_tree, from its sizes."""
+    """(rows of a tile, blocks that share a head's work, blocks of a cluster or 0, 32-bit words of work space) of a call of attention_tree, from its sizes."""
     slots = _decode_slots(device) // 3 * 2             # two blocks a multiprocessor
     if tensor_cores:
         rows_tile = 128 // group * group               # whole nodes in 128 rows
@@ -959,7 +972,8 @@ def _tree_plan(tensor_cores: bool, n_seqs: int, max_nodes: int, group: int, nkv:
         rows_tile = 32 if max_nodes * group > 16 and hd <= 256 else 16
     units = n_seqs * -(-max_nodes * group // rows_tile)
     shares = tree_shares(n_pages * units, units, min(rows_tile, max_nodes * group), nkv, slots)
-    return rows_tile, shares, 0 if shares == 1 else 2 * shares * nkv * rows_tile * (hd + 2) + 4 * nkv * min(shares - 1, units)
+    cluster = tree_cluster(n_pages, units, min(rows_tile, max_nodes * group), nkv, slots) if tensor_cores else 0
+    return rows_tile, shares, cluster, 0 if shares == 1 or cluster else 2 * shares * nkv * rows_tile * (hd + 2) + 4 * nkv * min(shares - 1, units)
 
 
 @_profiled(lambda a, facts: _attention_cost(a, facts))
@@ -999,17 +1013,19 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     one_sink, sinks = _sink(sink, nq)
     max_pages = block_table.shape[1]
     longest = max_pages if max_kv_len is None else max(1, min(max_pages, (int(max_kv_len) + PAGE - 1) // PAGE))
+    if window > 0:
+        longest = min(longest, (int(window) + max_nodes) // PAGE + 2 + (int(keep) + PAGE - 1) // PAGE)
     device = q.device
     pointers = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
     tensor_cores = dtype is torch.bfloat16 and hd in (64, 128, 256) and nq <= 128 * nkv and not \
         ((pointers[0] | pointers[1] | pointers[2] | pointers[3]) & 15 or (q_stride | o_stride) & 7)
-    rows_tile, shares, words_of_work = _tree_plan(tensor_cores, n_seqs, max_nodes, nq // nkv, nkv, hd, longest, device.index)
+    rows_tile, shares, cluster, words_of_work = _tree_plan(tensor_cores, n_seqs, max_nodes, nq // nkv, nkv, hd, longest, device.index)
     work = torch.empty(words_of_work, dtype=torch.float32, device=device) if words_of_work else None
     call = _TREE_CALL.pack(
         *pointers, block_table.data_ptr(), seq_slot.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
         _or_null(positions), sinks or 0, _or_null(work), status_word(device).data_ptr(),
         q_stride, o_stride, tokens, dtype_code(dtype), k_cache.shape[0], max_pages, words, n_seqs, max_nodes, nq, nkv, hd, int(window), int(keep),
-        shares, rows_tile, scale, one_sink, softcap)
+        shares, rows_tile, cluster, scale, one_sink, softcap)
     _check(_lib().rb_attention_tree(call, _stream()), "attention_tree")
 
 

@@ -132,6 +132,21 @@ def test_shares_fill_the_device_and_never_outnumber_the_pages():
     assert kernels.tree_shares(1, 1, 128, 5000, 296) == 1
 
 
+def test_clusters_stay_small_and_together_on_the_device():
+    for n_pages in (1, 2, 3, 8, 16, 17, 40, 41, 72, 73, 144, 145, 2000):
+        for units in (1, 2, 3, 8, 37, 1000):
+            for rows in (1, 16, 32, 33, 64, 128):
+                for nkv in (1, 3, 8, 16, 200):
+                    for slots in (148, 296):
+                        c = kernels.tree_cluster(n_pages, units, rows, nkv, slots)
+                        assert c in (0, 2, 4, 8, 16)
+                        if c:
+                            assert units * nkv * c <= slots and n_pages <= 9 * c and c // 2 < n_pages
+                            assert c < 16 or (rows <= 32 and 2 * units * nkv * c <= slots)
+    assert [kernels.tree_cluster(p, 1, 16, 8, 296) for p in (1, 2, 5, 16, 17, 144, 145)] == [0, 2, 8, 8, 16, 16, 0]
+    assert [kernels.tree_cluster(p, 1, 128, 8, 296) for p in (5, 40, 41)] == [8, 8, 0]
+
+
 def _attention(**change):
     """A call that is right but for living on the host."""
     i32 = torch.int32

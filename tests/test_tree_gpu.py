@@ -309,3 +309,23 @@ def test_tree_accept_a_whole_chain_of_256():
                         seq_slot=d["seq_slot"], kv_len=d["kv_len"], block_table=d["block_table"], k=k, v=v)
     assert path[0].tolist() == list(range(256)) and count.item() == 256 and drawn.item() == 256
     assert torch.equal(k.cpu(), t.k) and torch.equal(v.cpu(), t.v)
+
+
+@pytest.mark.parametrize("blocks", [0, 2, 4, 8, 16])
+@pytest.mark.parametrize("nq,nkv,hd", [(4, 2, 64), (8, 2, 128), (6, 2, 256), (16, 1, 64)])
+@pytest.mark.parametrize("sizes", list(SIZES))
+def test_attention_tree_blocks_of_a_cluster(blocks, nq, nkv, hd, sizes, monkeypatch):
+    """However many blocks share a sequence's pages, and joining by either way."""
+    from rocml_b200 import kernels
+    monkeypatch.setattr(kernels, "tree_cluster", lambda *a: blocks)
+    kernels._tree_plan.cache_clear()
+    try:
+        t = Trees(blocks + nq, SIZES[sizes], nq, nkv, hd, torch.bfloat16)
+        check(t, torch.bfloat16, call(t))
+        sinks = torch.linspace(-3.0, 2.0, nq)
+        options = dict(window=150, keep=20, softcap=8.0)
+        first = call(t, sink=sinks.to(DEV), **options)
+        check(t, torch.bfloat16, first, sinks=sinks, **options)
+        assert all(torch.equal(first, call(t, sink=sinks.to(DEV), **options)) for _ in range(20))
+    finally:
+        kernels._tree_plan.cache_clear()
