@@ -347,7 +347,7 @@ int rb_rglru_step(const float* u, int ld_u, const void* ra, const void* ri, int 
 // Attention of trees of drafted tokens over the paged cache (attention_tree.cu): sequence b's nodes are the rows cu_q[b] .. cu_q[b + 1], their keys
 // and values lie at the places kv_len[b] - n + j; row t sees the context (inside `window` of positions[t], and below `keep`) and the nodes whose
 // bits are set in visible[t] (int32 [tokens, words]).  shares: blocks that share a head's pages; rows_tile: 16 or 32, or 128 / group * group for
-// the tensor-core kernel.  cluster: 0, or (tensor-core kernel only) 2, 4, 8 or 16 blocks that share a sequence's tile of rows instead.
+// the tensor-core kernel.  cluster: 0, or (tensor-core kernel only) 2 to 16 blocks that share a sequence's tile of rows instead.
 typedef struct RbTreeCall {
     const void *q, *k_cache, *v_cache;
     void* out;

@@ -497,7 +497,7 @@ extern "C" int rb_attention_tree(const RbTreeCall* call, void* stream) {
     if (units > 0x7fffffff / MAX_SEQS) return RB_ERR_BAD_SIZE;
     a.max_units = (int)units;
     const bool clustered = x.cluster > 1;
-    if (clustered && (!tc5 || x.cluster > 16 || (x.cluster & (x.cluster - 1)) || x.n_seqs * units * x.cluster > 0x7fffffff)) return RB_ERR_BAD_SIZE;
+    if (clustered && (!tc5 || x.cluster > 16 || x.n_seqs * units * x.cluster > 0x7fffffff)) return RB_ERR_BAD_SIZE;
     a.cluster = x.cluster;
     if (x.shares > 1 && !clustered) {
         const size_t places = 2ull * x.shares * x.nkv * x.rows_tile;

@@ -952,12 +952,12 @@ def tree_cluster(n_pages: int, units: int, rows: int, nkv: int, slots: int) -> i
     """How many blocks of a cluster share a (sequence, tile of rows) and join what they found through each other's shared memory; 0: all heads' work is
     shared equally (``tree_shares``) and a second kernel joins.  The cluster saves that kernel and the way through memory but has few blocks, and every
     sequence costs what the longest does: it is taken while a block has few pages (8 heads, one sequence; us here and with two kernels: 4 rows, 300 keys
-    8.5 and 10.6, 3,000 keys 10.5 and 15.3; 64 rows, 1,000 keys 11.4 and 13.5, 6,000 keys 19.2 and 16.8; 128 rows, 1,000 keys 13.7 and 19.4; 8 sequences of
-    64 rows and 1,000 keys 15.4 and 19.2).  Sixteen blocks, which not every part of the device has beside others, only where half a device is enough and
-    rows are few (32 rows, 6,000 keys 14.4, with eight blocks 17.4; 128 rows, 1,000 keys 16.2 and 13.7)."""
-    blocks = 16 if rows <= 32 and n_pages > 16 and 32 * units * nkv <= slots else 8
-    while blocks > 1 and (units * nkv * blocks > slots or blocks // 2 >= n_pages):
-        blocks //= 2
+    8.5 and 10.6, 4,000 keys 11.7 and 15.2; 64 rows, 1,000 keys 10.7 and 13.8, 8,000 keys 19.2 and 17.0; 128 rows, 1,000 keys 14.5 and 19.4; 6 sequences
+    of 64 rows and 1,000 keys 14.9 and 17.8).  Seven blocks (more have more to join: 64 rows, 1,000 keys in 4, 7, 8 and 12 blocks 13.3, 10.7, 11.4 and
+    11.6 us); sixteen, which not every part of the device has beside others, only where half a device is enough and rows are few (16 rows, 4,000 keys
+    11.7, with seven 15.7).  An eighth of the device stays out: clusters do not fill it (4 sequences in clusters of 8 and 9: 14.3 and 23.5 us)."""
+    room = slots * 7 // 8 // (units * nkv)
+    blocks = min(16 if rows <= 32 and n_pages > 16 and 32 * units * nkv <= slots else 7, room, n_pages)
     return blocks if blocks > 1 and n_pages <= blocks * (5 if rows > 32 else 9) else 0
 
 

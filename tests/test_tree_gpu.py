@@ -311,7 +311,7 @@ def test_tree_accept_a_whole_chain_of_256():
     assert torch.equal(k.cpu(), t.k) and torch.equal(v.cpu(), t.v)
 
 
-@pytest.mark.parametrize("blocks", [0, 2, 4, 8, 16])
+@pytest.mark.parametrize("blocks", [0, 2, 5, 7, 16])
 @pytest.mark.parametrize("nq,nkv,hd", [(4, 2, 64), (8, 2, 128), (6, 2, 256), (16, 1, 64)])
 @pytest.mark.parametrize("sizes", list(SIZES))
 def test_attention_tree_blocks_of_a_cluster(blocks, nq, nkv, hd, sizes, monkeypatch):
