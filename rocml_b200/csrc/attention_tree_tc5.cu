@@ -121,8 +121,8 @@ __device__ __forceinline__ void join_cluster(const TreeArgs& a, const ClusterSha
             for (int e = 0; e < 4; ++e) acc[e] *= old;
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
-                const float w = c0 + j < share.parts ? exp2f(m[j] - top) : 0.f;
-                if (w == 0.f) continue;                      // (past the last part, or nothing beside the others)
+                if (c0 + j >= share.parts) continue;         // (a part of weight zero is added all the same: it may be NaN)
+                const float w = exp2f(m[j] - top);
                 total = fmaf(l[j], w, total);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[e] = fmaf(x[j][e], w, acc[e]);

@@ -1,0 +1,47 @@
+"""Trees of drafted tokens and scoring at the edges of what a call allows: keys that are not finite, positions past the sequence's last place,
+sequences without nodes, rows without enough finite logits."""
+import math
+
+import pytest
+import torch
+
+import plain_tree
+from plain_tree import Trees
+from test_tree_gpu import DEV, bound, call, check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def cluster_of(monkeypatch):
+    """Sets how many blocks share a sequence's pages in the tensor-core kernel (0: equal shares and a second kernel; None: by the rule)."""
+    from rocml_b200 import kernels
+
+    def choose(blocks):
+        if blocks is not None:
+            monkeypatch.setattr(kernels, "tree_cluster", lambda *a: blocks)
+        kernels._tree_plan.cache_clear()
+    yield choose
+    kernels._tree_plan.cache_clear()
+
+
+@pytest.mark.parametrize("dtype,nq,nkv,hd,blocks", [(torch.bfloat16, q, n, h, b) for q, n, h in ((8, 2, 128), (16, 1, 64), (6, 2, 256)) for b in (0, 2, 7, 16)]
+                         + [(torch.float32, 4, 2, 64, None), (torch.bfloat16, 4, 2, 48, None)])
+def test_keys_that_are_not_finite_reach_the_rows_that_see_them(dtype, nq, nkv, hd, blocks, cluster_of):
+    """Pages of nothing but NaN keys, whichever block they fall to: NaN in the rows that see them, the same bits in the others."""
+    cluster_of(blocks)
+    t = Trees(41 + hd, [(700, 33), (640, 128), (190, 9)], nq, nkv, hd, dtype)
+    want = call(t)
+    assert torch.isfinite(want).all()
+    kept = t.k.clone()
+    for places in ([192], range(0, 384, 64)):          # inside the first sequence's context, one page and half of them: all its rows
+        for p in places:
+            t.k[0, t.place(0, p)[0]] = math.nan
+        out = call(t)
+        assert torch.isnan(out[:t.cu[1]]).all() and torch.equal(out[t.cu[1]:], want[t.cu[1]:])
+        t.k = kept.clone()
+    t.k[0, t.place(1, 704)[0]] = math.nan              # the second sequence's nodes 64 to 127: themselves
+    out = call(t)
+    hit = slice(t.cu[1] + 64, t.cu[2])
+    assert torch.isnan(out[hit]).all()
+    assert torch.equal(out[:hit.start], want[:hit.start]) and torch.equal(out[hit.stop:], want[hit.stop:])
