@@ -145,9 +145,13 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
 #pragma unroll 1
         for (int i = 0; i < RING - 1; ++i) fetch(i);
         RowBits bits[RPT];
+        int ahead = 0;                                 // the furthest position of this thread's rows
 #pragma unroll
         for (int r = 0; r < RPT; ++r)
-            if (RPT * rg + r < rows) bits[r].load(a, s.q0 + (row0 + RPT * rg + r) / a.group);
+            if (RPT * rg + r < rows) {
+                bits[r].load(a, s.q0 + (row0 + RPT * rg + r) / a.group);
+                ahead = max(ahead, bits[r].position);
+            }
         float m[RPT], l[RPT], o[BLOCKS][RPT][4];
 #pragma unroll
         for (int r = 0; r < RPT; ++r) {
@@ -161,8 +165,8 @@ attention_tree_simple_kernel(const T* __restrict__ q, long long q_stride, T* __r
         int block = 0;
         for (int j = p0; j < p1; ++j) {
             const int key0 = tile_of(s, j) * PAGE;
-            // a tile inside the context that every row sees whole needs no mask (no position is behind the sequence's last)
-            const bool whole_tile = key0 + PAGE <= s.ctx && (a.window == 0 || key0 >= s.len - a.window || key0 + PAGE <= a.keep);
+            // a tile inside the context that each of these rows sees whole needs no mask
+            const bool whole_tile = key0 + PAGE <= s.ctx && (a.window == 0 || key0 > ahead - a.window || key0 + PAGE <= a.keep);
             float sc[RPT][4] = {};
 #pragma unroll 1
             for (int c = 0; c < BLOCKS; ++c) {

@@ -322,11 +322,16 @@ attention_tree_tc5_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             float m_used = NEG_BIG, l_sum = 0.f;
             RowBits bits;
             if (row_here) bits.load(a, s.q0 + node);
+            int ahead = 0;                           // the furthest position of the tile's nodes, of which a tile has 128 at most
+            if (a.window > 0) {
+                for (int i = lane; i < rows / a.group; i += 32) ahead = max(ahead, a.positions[s.q0 + row0 / a.group + i]);
+                ahead = __reduce_max_sync(0xffffffffu, ahead);
+            }
             for (int j = p0; j < p1; ++j, ++it) {
                 const int buf = it & 1, st = it % STAGES;
                 const int key0 = tile_of(s, j) * BK;
-                // a tile inside the context that every node sees whole needs no mask (no position is behind the sequence's last)
-                const bool whole_tile = key0 + BK <= s.ctx && (a.window == 0 || key0 >= s.len - a.window || key0 + BK <= a.keep);
+                // a tile inside the context that every node sees whole needs no mask
+                const bool whole_tile = key0 + BK <= s.ctx && (a.window == 0 || key0 > ahead - a.window || key0 + BK <= a.keep);
                 unsigned long long seen = ~0ull;
                 bool spoiled = false;
                 // This wait comes before the one for V: scores of this tile say that the product of the tile before last is done, and so that the V before

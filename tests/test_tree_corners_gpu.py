@@ -45,3 +45,12 @@ def test_keys_that_are_not_finite_reach_the_rows_that_see_them(dtype, nq, nkv, h
     hit = slice(t.cu[1] + 64, t.cu[2])
     assert torch.isnan(out[hit]).all()
     assert torch.equal(out[:hit.start], want[:hit.start]) and torch.equal(out[hit.stop:], want[hit.stop:])
+
+
+@pytest.mark.parametrize("window,keep", [(1, 0), (64, 3), (100, 70), (300, 0)])
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 48), (torch.bfloat16, 128), (torch.bfloat16, 64)])
+def test_positions_past_the_sequences_last_place(window, keep, dtype, hd):
+    """A window goes by a node's position, wherever that is: none of the context may be left of it."""
+    t = Trees(window + hd, [(700, 33), (3, 5), (128, 20), (2050, 12)], 4, 2, hd, dtype)
+    t.positions = t.positions + torch.arange(t.cu[-1], dtype=torch.int32) * 37 % 250
+    check(t, dtype, call(t, window=window, keep=keep), window=window, keep=keep)
