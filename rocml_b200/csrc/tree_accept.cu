@@ -32,7 +32,7 @@ tree_accept_kernel(const int* __restrict__ tokens, const int* __restrict__ paren
     const int b = blockIdx.y, tid = threadIdx.x;
     const int slot = seq_slot ? seq_slot[b] : 0, q0 = cu_q[b];
     const int n = min(min(cu_q[b + 1] - q0, words * 32), path_ld);
-    if (slot < 0 || n <= 0) return;
+    if (slot < 0) return;                                // (a sequence without nodes has a path of none)
     first[tid] = MAX_NODES;
     way[tid] = -1;
     if (tid == 0) count = 0;

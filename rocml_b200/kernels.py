@@ -1037,7 +1037,8 @@ def tree_accept(token_ids: torch.Tensor, parents: torch.Tensor, visible: torch.T
     """What of every tree of drafted tokens (int32 ``token_ids``, ``parents`` within the tree, -1 for the first node and any other root, and the
     rows of ancestor bits ``visible``) the tokens that were sampled at the nodes confirm.  Node 0 always is; a node below it when its parent is
     and the parent's sampled token is its own (of several such children the first).  path int32 [n_seqs, >= the largest tree] receives the confirmed
-    nodes from node 0 down, -1 behind them, counts [n_seqs] how many they are, next_token [n_seqs] the token sampled at the last one.
+    nodes from node 0 down, -1 behind them, counts [n_seqs] how many they are, next_token [n_seqs] the token sampled at the last one (0 and -1 where a
+    sequence brings no node).
     With ``k`` and ``v`` [layers, pages, nkv, 64, hd] (``v`` None: one tensor serves as both; and seq_slot, kv_len, block_table as for
     ``attention_tree``) their keys and values are moved
     to the places kv_len - n + 0, 1, 2, ... in every layer.  Rows of slots below 0 stay as they are.  Parents come before their

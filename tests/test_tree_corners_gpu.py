@@ -54,3 +54,17 @@ def test_positions_past_the_sequences_last_place(window, keep, dtype, hd):
     t = Trees(window + hd, [(700, 33), (3, 5), (128, 20), (2050, 12)], 4, 2, hd, dtype)
     t.positions = t.positions + torch.arange(t.cu[-1], dtype=torch.int32) * 37 % 250
     check(t, dtype, call(t, window=window, keep=keep), window=window, keep=keep)
+
+
+def test_a_sequence_without_nodes_has_nothing_confirmed():
+    from rocml_b200 import kernels
+    t = Trees(5, [(30, 3), (64, 1), (10, 4)], 1, 1, 16, torch.bfloat16)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    d = t.ints(DEV)
+    cu, lens = i32([0, 3, 3, 7]), i32([33, 64, 14])
+    visible = torch.cat([plain_tree.bits_of(p, 1) for p in ([-1, 0, 1], [-1, 0, 0, 1])]).to(DEV)
+    k, v = t.k.to(DEV), t.v.to(DEV)
+    path, counts, drawn = torch.full((3, 5), 9, dtype=torch.int32, device=DEV), i32([9] * 3), i32([9] * 3)
+    kernels.tree_accept(i32([4, 5, 6, 4, 8, 5, 7]), i32([-1, 0, 1, -1, 0, 0, 1]), visible, i32([5, 6, 1, 5, 3, 2, 0]), cu, 3, path, counts, drawn,
+                        seq_slot=d["seq_slot"], kv_len=lens, block_table=d["block_table"], k=k, v=v)
+    assert path.tolist() == [[0, 1, 2, -1, -1], [-1] * 5, [0, 2, -1, -1, -1]] and counts.tolist() == [3, 0, 2] and drawn.tolist() == [1, -1, 2]
