@@ -427,7 +427,8 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, int V, const i
     if ((int)threadIdx.x < top) {
         const Key k = sh.best[threadIdx.x];
         if (top_ids) top_ids[(size_t)r * top + threadIdx.x] = k ? key_index(k) : -1;
-        if (top_logprobs) top_logprobs[(size_t)r * top + threadIdx.x] = !k || nothing ? -INFINITY : logprob(key_value(k));
+        // (too few candidates: the row holds NaN, which is nobody's candidate and has spoiled the sums)
+        if (top_logprobs) top_logprobs[(size_t)r * top + threadIdx.x] = nothing ? -INFINITY : k ? logprob(key_value(k)) : total;
     }
 }
 }  // namespace

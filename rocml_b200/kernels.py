@@ -1098,7 +1098,7 @@ def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor], logprobs: 
     receives those of the tokens ids int32 [n, m] (-inf for an id outside the vocabulary), entropy float32 [n] the rows' entropy,
     top_logprobs float32 and top_ids int32 [n, k], k <= 32, the k most likely tokens, most likely first, equal ones by their id.  Any of the three may be
     None.  A logit of -inf is a token that cannot be; in a row of nothing else every log probability is -inf and the entropy 0.  A row that holds a NaN
-    or +inf gives NaN."""
+    or +inf gives NaN (its alternatives are those of the logits that are numbers, -1 where there are too few)."""
     if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < 1:
         raise KernelError("token_logprobs: logits must be [n, V] with unit inner stride")
     n, V = logits.shape

@@ -68,3 +68,18 @@ def test_a_sequence_without_nodes_has_nothing_confirmed():
     kernels.tree_accept(i32([4, 5, 6, 4, 8, 5, 7]), i32([-1, 0, 1, -1, 0, 0, 1]), visible, i32([5, 6, 1, 5, 3, 2, 0]), cu, 3, path, counts, drawn,
                         seq_slot=d["seq_slot"], kv_len=lens, block_table=d["block_table"], k=k, v=v)
     assert path.tolist() == [[0, 1, 2, -1, -1], [-1] * 5, [0, 2, -1, -1, -1]] and counts.tolist() == [3, 0, 2] and drawn.tolist() == [1, -1, 2]
+
+
+@pytest.mark.parametrize("V,top", [(1, 1), (3, 3), (3000, 5), (40000, 32)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_alternatives_of_a_row_that_holds_nan_are_nan(V, top, dtype):
+    """However few of its logits are numbers."""
+    from rocml_b200 import kernels
+    x = torch.full((4, V), math.nan, dtype=dtype)
+    x[1, :V // 2] = 1.0
+    x[2, 1:] = torch.randn(V - 1, generator=torch.Generator().manual_seed(V)).to(dtype)
+    x[3] = -math.inf
+    values, ids = torch.full((4, top), 9.0, device=DEV), torch.full((4, top), 9, dtype=torch.int32, device=DEV)
+    kernels.token_logprobs(x.to(DEV), None, None, None, values, ids)
+    assert torch.isnan(values[:3]).all() and torch.isneginf(values[3]).all()
+    assert (ids[0] == -1).all() and ids[3].tolist() == list(range(top)) and ((ids >= -1) & (ids < V)).all()
