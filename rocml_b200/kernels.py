@@ -1008,7 +1008,7 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     if seq_slot.numel() < n_seqs or kv_len.numel() < n_seqs or block_table.dim() != 2:
         raise KernelError("attention_tree: seq_slot, kv_len and block_table do not fit")
     _ints_here("attention_tree", (block_table, seq_slot, cu_q, kv_len, visible, positions), (q, out, k_cache, v_cache))
-    if n_seqs == 0:
+    if n_seqs == 0 or tokens == 0:
         return
     one_sink, sinks = _sink(sink, nq)
     max_pages = block_table.shape[1]

@@ -83,3 +83,15 @@ def test_alternatives_of_a_row_that_holds_nan_are_nan(V, top, dtype):
     kernels.token_logprobs(x.to(DEV), None, None, None, values, ids)
     assert torch.isnan(values[:3]).all() and torch.isneginf(values[3]).all()
     assert (ids[0] == -1).all() and ids[3].tolist() == list(range(top)) and ((ids >= -1) & (ids < V)).all()
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 128)])
+def test_a_call_without_a_single_node(dtype, hd):
+    from rocml_b200 import kernels
+    t = Trees(6, [(70, 2), (5, 3)], 4, 2, hd, dtype)
+    d = t.ints(DEV)
+    q, out = torch.zeros((0, 4 * hd), dtype=dtype, device=DEV), torch.full((5, 4 * hd), 7.0, dtype=dtype, device=DEV)
+    kernels.attention_tree(q, out, t.k[0].to(DEV), t.v[0].to(DEV), d["block_table"], d["seq_slot"], torch.zeros_like(d["cu_q"]), d["kv_len"],
+                           d["visible"][:0], 2, 1, 4, 2, hd, 0.1)
+    kernels.check_status(DEV)
+    assert (out == 7).all()
