@@ -483,7 +483,7 @@ extern "C" int rb_attention_tree(const RbTreeCall* call, void* stream) {
     const RbTreeCall& x = *call;
     if (x.n_seqs <= 0 || x.max_nodes <= 0) return RB_OK;
     if (x.n_seqs > MAX_SEQS || x.nkv <= 0 || x.nq <= 0 || x.nq % x.nkv || x.hd <= 0 || x.hd > 512 || x.words <= 0 || x.max_nodes > 32 * x.words ||
-        x.shares <= 0 || x.shares > 32767 || x.window < 0 || x.keep < 0 || !(x.scale > 0.f) || x.max_pages <= 0 || (x.window > 0 && !x.positions) ||
+        x.shares <= 0 || x.shares > 32767 || x.window < 0 || x.keep < 0 || !(x.scale > 0.f) || x.max_pages <= 0 || x.max_pages > 0x7fffffff / PAGE || (x.window > 0 && !x.positions) ||
         (x.shares > 1 && x.cluster <= 1 && !x.work) || x.nkv > 65535 || x.rows_tile <= 0)
         return RB_ERR_BAD_SIZE;
     if (x.dtype != RB_F32 && x.dtype != RB_BF16) return RB_ERR_BAD_DTYPE;
@@ -495,7 +495,7 @@ extern "C" int rb_attention_tree(const RbTreeCall* call, void* stream) {
     a.block_table = x.block_table; a.max_pages = x.max_pages; a.seq_slot = x.seq_slot; a.cu_q = x.cu_q; a.kv_len = x.kv_len;
     a.visible = x.visible; a.words = x.words; a.positions = x.positions;
     a.B = x.n_seqs; a.nq = x.nq; a.nkv = x.nkv; a.group = group; a.hd = x.hd;
-    a.scale = x.scale; a.window = x.window; a.keep = x.window > 0 ? x.keep : 0; a.sink = x.sink; a.sinks = x.sinks; a.softcap = x.softcap;
+    a.scale = x.scale; a.window = x.window; a.keep = x.window <= 0 ? 0 : x.keep / PAGE < x.max_pages ? x.keep : x.max_pages * PAGE; a.sink = x.sink; a.sinks = x.sinks; a.softcap = x.softcap;
     a.shares = x.shares; a.rows_tile = x.rows_tile; a.max_nodes = x.max_nodes;
     const long long units = ((long long)x.max_nodes * group + x.rows_tile - 1) / x.rows_tile;
     if (units > 0x7fffffff / MAX_SEQS) return RB_ERR_BAD_SIZE;

@@ -1012,9 +1012,10 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         return
     one_sink, sinks = _sink(sink, nq)
     max_pages = block_table.shape[1]
+    window, keep = min(int(window), 2 ** 31 - 1), min(int(keep), max_pages * PAGE)       # (more than a row of the table holds is all of it)
     longest = max_pages if max_kv_len is None else max(1, min(max_pages, (int(max_kv_len) + PAGE - 1) // PAGE))
     if window > 0:
-        longest = min(longest, (int(window) + max_nodes) // PAGE + 2 + (int(keep) + PAGE - 1) // PAGE)
+        longest = min(longest, (window + max_nodes) // PAGE + 2 + (keep + PAGE - 1) // PAGE)
     device = q.device
     pointers = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
     tensor_cores = dtype is torch.bfloat16 and hd in (64, 128, 256) and nq <= 128 * nkv and not \
@@ -1024,7 +1025,7 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     call = _TREE_CALL.pack(
         *pointers, block_table.data_ptr(), seq_slot.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(), visible.data_ptr(),
         _or_null(positions), sinks or 0, _or_null(work), status_word(device).data_ptr(),
-        q_stride, o_stride, tokens, dtype_code(dtype), k_cache.shape[0], max_pages, words, n_seqs, max_nodes, nq, nkv, hd, int(window), int(keep),
+        q_stride, o_stride, tokens, dtype_code(dtype), k_cache.shape[0], max_pages, words, n_seqs, max_nodes, nq, nkv, hd, window, keep,
         shares, rows_tile, cluster, scale, one_sink, softcap)
     _check(_lib().rb_attention_tree(call, _stream()), "attention_tree")
 

@@ -95,3 +95,12 @@ def test_a_call_without_a_single_node(dtype, hd):
                            d["visible"][:0], 2, 1, 4, 2, hd, 0.1)
     kernels.check_status(DEV)
     assert (out == 7).all()
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 48), (torch.bfloat16, 128)])
+def test_as_many_kept_places_as_an_integer_holds(dtype, hd):
+    """More than the context has: the whole of it is kept, as without a window."""
+    t = Trees(7, [(700, 33), (3, 5), (128, 20)], 4, 2, hd, dtype)
+    for keep in (2 ** 31 - 1, 2 ** 31 - 64, 2 ** 20):
+        check(t, dtype, call(t, window=5, keep=keep), window=5, keep=keep)
+    check(t, dtype, call(t, window=2 ** 31 - 1, keep=2 ** 31 - 1))
