@@ -1007,7 +1007,8 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         raise KernelError("attention_tree: scale is positive, window, keep and softcap are not negative, a window comes with positions")
     if seq_slot.numel() < n_seqs or kv_len.numel() < n_seqs or block_table.dim() != 2:
         raise KernelError("attention_tree: seq_slot, kv_len and block_table do not fit")
-    _ints_here("attention_tree", (block_table, seq_slot, cu_q, kv_len, visible, positions), (q, out, k_cache, v_cache))
+    _ints_here("attention_tree", (block_table, seq_slot, cu_q, kv_len, visible, positions),
+               (q, out, k_cache, v_cache, sink if isinstance(sink, torch.Tensor) else None))
     if n_seqs == 0 or tokens == 0:
         return
     one_sink, sinks = _sink(sink, nq)
