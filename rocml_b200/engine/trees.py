@@ -77,6 +77,9 @@ class TreeSteps:
         self.engine = engine
         # (a step's logits, one row a node, stay within the head room of the engine's memory budget)
         self.max_nodes = min(engine.max_step_tokens, max(2 * MAX_NODES, engine.cache.max_slots))
+        # A node sees all its ancestors: they must lie in every layer's window (its own, whatever the cache keeps for another layer that reads it).
+        own = [b.mixer.cache_requirement() for b in engine.model.blocks]
+        self.max_depth = min([MAX_NODES] + [int(r.window) for r in own if getattr(r, "window", None)])
         self._buffers = {}
         self._sampler = None
 
@@ -91,9 +94,8 @@ class TreeSteps:
             if len(e.tokens) > self.max_nodes:
                 raise RocmlError(f"slot {e.slot}: a tree of {len(e.tokens)} nodes; a step holds {self.max_nodes}")
             depth = max(pack_trees([0], [e.parents])[0]) + 1
-            spans = [g.req.window for g in self.engine.cache.kv_groups if g.req.window is not None]
-            if spans and depth > min(spans):
-                raise RocmlError(f"slot {e.slot}: a tree {depth} nodes deep; a layer's window holds {min(spans)} positions")
+            if depth > self.max_depth:
+                raise RocmlError(f"slot {e.slot}: a tree {depth} nodes deep; a layer's window holds {self.max_depth} positions")
         # room for everything, before anything launches (every tree beside all others, as if none gave a page back)
         self.engine.cache.plan([[(e.slot, len(e.tokens)) for e in entries]])
         return entries

@@ -13,6 +13,28 @@ from rocml_b200.cache import SequenceCache
 from rocml_b200.errors import KernelError, RocmlError
 
 
+@pytest.mark.parametrize("keeper,reader,deepest", [(50, 7, 7), (9, 50, 9), (None, 8, 8), (12, None, 12), (None, None, 256)])
+def test_the_narrowest_window_of_any_layer_bounds_a_tree(keeper, reader, deepest):
+    """Also where the cache keeps more, for another layer that reads it."""
+    from rocml_b200.config import config_from_dict
+    from rocml_b200.engine.model import Model
+    from rocml_b200.engine.trees import TreeEntry, TreeSteps
+    from rocml_b200.parts import BuildEnv
+    from tiny_models import _KA_ROT, _kdiff
+    cfg = {"architecture": "Kemizen", "vocab": 211, "width": 64, "embedding": {"scale": 1.5}, "norm": {"eps": 1e-6},
+           "layers": [_kdiff(4, 2, 12, 20, 0.5, 0.3, _KA_ROT, 96, size=keeper), _kdiff(4, 2, 12, 20, 0.7, 0.5, _KA_ROT, 48, size=reader, kv_from=0)]}
+    model = Model(config_from_dict(cfg).to_model_spec(), BuildEnv(torch.device("cpu"), torch.float32))
+    cache = SequenceCache(model.cache_requirements(), model.reads_cache_of(), 1024, 2, 1024, torch.float32, torch.device("cpu"), 512)
+    steps = TreeSteps(SimpleNamespace(model=model, cache=cache, max_step_tokens=512))
+    slot = cache.alloc_slot()
+    chain = lambda n: TreeEntry(slot, [1] * n, list(range(-1, n - 1)))
+    assert steps._check([chain(deepest)])
+    assert steps._check([TreeEntry(slot, [1] * 200, [-1] + [0] * 199)])
+    if deepest < 256:
+        with pytest.raises(RocmlError, match=f"window holds {deepest} positions"):
+            steps._check([chain(deepest + 1)])
+
+
 class _OnAnotherDevice(torch.Tensor):
     def get_device(self):
         return 5
