@@ -103,7 +103,7 @@ class TreeSteps:
     def _pieces(self, entries):
         cur, n = [], 0
         for e in entries:
-            if cur and n + len(e.tokens) > self.max_nodes:
+            if cur and (n + len(e.tokens) > self.max_nodes or len(cur) == kernels.TREE_MAX_SEQS):
                 yield cur
                 cur, n = [], 0
             cur.append(e)

@@ -35,6 +35,16 @@ def test_the_narrowest_window_of_any_layer_bounds_a_tree(keeper, reader, deepest
             steps._check([chain(deepest + 1)])
 
 
+def test_a_step_takes_no_more_sequences_than_its_kernels():
+    from rocml_b200.engine.trees import TreeEntry, TreeSteps
+    steps = TreeSteps.__new__(TreeSteps)
+    steps.max_nodes = 4096
+    entries = [TreeEntry(i, [1] * (1 + i % 3 // 2), [-1, 0][:1 + i % 3 // 2]) for i in range(2500)]
+    pieces = list(steps._pieces(entries))
+    assert [e for p in pieces for e in p] == entries and all(0 < len(p) <= kernels.TREE_MAX_SEQS for p in pieces)
+    assert all(sum(len(e.tokens) for e in p) <= 4096 for p in pieces) and len(pieces) == 3
+
+
 class _OnAnotherDevice(torch.Tensor):
     def get_device(self):
         return 5
