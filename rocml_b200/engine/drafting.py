@@ -52,13 +52,30 @@ class PromptLookup:
         return tokens, parents
 
 
-def _entry(slot: int, history: Sequence[int], drafter: Drafter, room: int) -> TreeEntry:
-    """The sequence's last token and the drafter's guesses below it, as many as there is room for (their parents come first)."""
+def _cut(tokens, parents, most: int, deepest: int) -> Tuple[List[int], List[int]]:
+    """The first ``most`` of the guesses that lie no deeper than ``deepest`` below the sequence's last token, parents renumbered."""
+    kept, ups, place, depth = [], [], {-1: -1}, {-1: 0}
+    for i, (token, up) in enumerate(zip(tokens, parents)):
+        if len(kept) >= most:
+            break
+        if not -1 <= up < i:
+            raise RocmlError(f"the drafter's guess {i} follows guess {up}: it must be -1 or an earlier one")
+        depth[i] = depth[up] + 1
+        if depth[i] <= deepest:
+            place[i] = len(kept)
+            kept.append(token)
+            ups.append(place[up])
+    return kept, ups
+
+
+def _entry(slot: int, history: Sequence[int], drafter: Drafter, room: int, nodes: int, depth: int) -> TreeEntry:
+    """The sequence's last token and the drafter's guesses below it, as many as there is room for and as a tree may have, ``nodes`` of them and
+    ``depth`` on a path (their parents come first, so what a guess follows is kept with it)."""
     tokens, parents = drafter(history)
     if len(tokens) != len(parents):
         raise RocmlError(f"the drafter gave {len(tokens)} tokens and {len(parents)} parents")
-    n = max(0, min(len(tokens), room - 1, MAX_NODES - 1))
-    return TreeEntry(slot, [history[-1]] + list(tokens[:n]), [-1] + [int(p) + 1 for p in parents[:n]])
+    tokens, parents = _cut(tokens, [int(p) for p in parents], min(room, nodes) - 1, depth - 1)
+    return TreeEntry(slot, [history[-1]] + tokens, [-1] + [p + 1 for p in parents])
 
 
 def generate_drafted(engine, requests: Sequence[Request], drafter: Drafter, default_stop: Iterable[int] = (), max_batch: int = 64,
@@ -88,6 +105,10 @@ def generate_drafted(engine, requests: Sequence[Request], drafter: Drafter, defa
             live.append({"i": i, "req": r, "slot": engine.new_sequence(), "out": [], "history": list(r.prompt), "need": needs[i],
                          "stops": default_stop if r.stop_tokens is None else set(r.stop_tokens), "rng": XorShift64Star(r.sampling.seed + j)})
 
+        def entry(s) -> TreeEntry:
+            nodes, depth = getattr(engine, "tree_limits", (MAX_NODES, MAX_NODES))
+            return _entry(s["slot"], s["history"], drafter, s["need"] - len(s["history"]) + 1, nodes, depth)
+
         def take(s, tokens) -> bool:
             """Append what was sampled; whether the sequence goes on."""
             r = s["req"]
@@ -105,7 +126,7 @@ def generate_drafted(engine, requests: Sequence[Request], drafter: Drafter, defa
             return True
 
         try:
-            _run_batch(engine, live, drafter, take, stats)
+            _run_batch(engine, live, entry, take, stats)
         except BaseException:
             for s in live:                    # (a drafter may fail: the sequences that were running give their slots back)
                 if results[s["i"]] is None:
@@ -114,8 +135,8 @@ def generate_drafted(engine, requests: Sequence[Request], drafter: Drafter, defa
     return results
 
 
-def _run_batch(engine, live, drafter, take, stats) -> None:
-    """Prompts, then drafts until every sequence has ended."""
+def _run_batch(engine, live, entry, take, stats) -> None:
+    """Prompts, then drafts (``entry`` of a sequence) until every sequence has ended."""
     first = True
     while live:
         t0 = time.perf_counter()
@@ -124,8 +145,7 @@ def _run_batch(engine, live, drafter, take, stats) -> None:
             sampled = [[t] for t in engine.run([s["slot"] for s in live], [s["history"] for s in live], [s["req"].sampling for s in live],
                                                [s["rng"] for s in live], [s["history"] for s in live])]
         else:
-            entries = [_entry(s["slot"], s["history"], drafter, s["need"] - len(s["history"]) + 1) for s in live]
-            sampled = engine.verify(entries, [s["req"].sampling for s in live], [s["rng"] for s in live], [s["history"] for s in live])
+            sampled = engine.verify([entry(s) for s in live], [s["req"].sampling for s in live], [s["rng"] for s in live], [s["history"] for s in live])
         running = live
         live = [s for s, tokens in zip(running, sampled) if take(s, tokens)]
         dt = time.perf_counter() - t0

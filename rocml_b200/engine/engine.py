@@ -480,6 +480,13 @@ class Engine:
             self._trees = TreeSteps(self)
         return self._trees
 
+    @property
+    def tree_limits(self) -> Tuple[int, int]:
+        """How many nodes a tree of drafted tokens may have here, and how many of them a path."""
+        from .trees import MAX_NODES
+        steps = self._tree_steps()
+        return min(steps.max_nodes, MAX_NODES), steps.max_depth
+
     def tree_logits(self, entries) -> torch.Tensor:
         """Float32 logits [all nodes, vocab] of trees of drafted tokens (``TreeEntry``), every node behind its sequence's context and its
         ancestors.  The sequences stay as long as they were.  The tensor may be reused by the next step."""

@@ -35,6 +35,50 @@ def test_the_narrowest_window_of_any_layer_bounds_a_tree(keeper, reader, deepest
             steps._check([chain(deepest + 1)])
 
 
+def test_an_engines_limits_cut_drafts():
+    """The loop's decisions with an engine that says what a tree may be: the ordinary answers, never more nodes or deeper ones."""
+    from rocml_b200.engine.drafting import generate_drafted
+    from rocml_b200.engine.generate import Request, generate
+    from rocml_b200.sampling import SamplingParams
+    from test_drafting import Fake
+
+    class Limited(Fake):
+        def verify(self, entries, params, rngs, histories):
+            for e in entries:
+                depth = []
+                for p in e.parents:
+                    depth.append(depth[p] + 1 if p >= 0 else 1)
+                assert len(e.tokens) <= self.tree_limits[0] and max(depth) <= self.tree_limits[1]
+                self.deepest = max(self.deepest, max(depth))
+            return super().verify(entries, params, rngs, histories)
+
+    for limits in ((1, 256), (2, 256), (9, 3), (256, 1), (256, 2), (30, 30)):
+        rng = random.Random(sum(limits))
+        reqs = [Request([rng.randrange(10) for _ in range(rng.randrange(1, 20))], 25, SamplingParams(), stop_tokens=[]) for _ in range(5)]
+
+        def drafter(history):
+            text, tokens, parents, above = list(history), [], [], -1
+            for _ in range(40):
+                guess = Fake.follow(text)
+                for g in ([guess, rng.randrange(11)] if rng.random() < 0.5 else [rng.randrange(11), guess]):
+                    tokens.append(g)
+                    parents.append(above)
+                above = next(i for i in range(len(tokens)) if parents[i] == above and tokens[i] == guess)
+                text.append(guess)
+            return tokens, parents
+        plain, limited = Fake(), Limited()
+        limited.tree_limits, limited.deepest = limits, 0
+        want, got = generate(plain, reqs, max_batch=3), generate_drafted(limited, reqs, drafter, max_batch=3)
+        assert [(c.tokens, c.finish_reason) for c in got] == [(c.tokens, c.finish_reason) for c in want]
+        assert max(limited.nodes) <= limits[0] and (limited.steps < plain.steps) == (min(limits) > 1)
+        assert limited.deepest == 1 if min(limits) == 1 else limited.deepest > 1
+    for parents in ([-1, 1], [-1, 5], [-2, 0]):
+        fake = Fake()
+        with pytest.raises(RocmlError, match="earlier"):
+            generate_drafted(fake, [Request([1, 2, 3], 5)], lambda h: ([1, 2], parents))
+        assert not fake.text
+
+
 def test_a_step_takes_no_more_sequences_than_its_kernels():
     from rocml_b200.engine.trees import TreeEntry, TreeSteps
     steps = TreeSteps.__new__(TreeSteps)

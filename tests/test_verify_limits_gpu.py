@@ -11,6 +11,32 @@ from tiny_models import _dense, _latent, _layer, prompt, write_pipilix
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("name,step_tokens", [("A", 4), ("A", 1), ("B", 20), ("C", 4096), ("E", 7), ("PA", 4096), ("PB", 12), ("PC", 4096)])
+def test_drafts_that_an_engine_cannot_take_are_cut(folders, name, step_tokens):        # noqa: F811
+    """More guesses than a step holds, deeper ones than a window: the answers are the ordinary ones (32-bit), also where no guess is left."""
+    from rocml_b200 import Engine, SamplingParams
+    vocab = vocab_of(name)
+    eng = Engine.from_folder(folders(name), dtype="float32", max_tokens=64 * 12, max_slots=3, max_step_tokens=step_tokens)
+    prompts = [prompt(60 + n, n, vocab) for n in (3, 17, 40)]
+    params = SamplingParams(0.8, 40, 0.95, seed=5)
+    want = eng.generate(prompts, max_new_tokens=14, sampling=params, stop_tokens=[])
+    texts = [p + w.tokens for p, w in zip(prompts, want)]
+
+    def drafter(history):
+        text = next(t for t in texts if t[:len(history)] == list(history))
+        guesses = (text[len(history):] + [1] * 40)[:40]
+        tokens, parents, above = [], [], -1
+        for g in guesses:                              # a chain of forty, each with a wrong guess beside it
+            tokens += [(g + 1) % vocab, g]
+            parents += [above, above]
+            above = len(tokens) - 1
+        return tokens, parents
+    got = eng.generate(prompts, max_new_tokens=14, sampling=params, stop_tokens=[], drafter=drafter)
+    assert [(g.tokens, g.finish_reason) for g in got] == [(w.tokens, w.finish_reason) for w in want]
+    eng.cache.check_invariants()
+    assert eng.cache.slots.n_held == 0
+
+
 @pytest.mark.parametrize("windows", [(50, 7), (9, 50), (None, 12)])
 def test_layers_that_read_anothers_cache_through_another_window(tmp_path, windows):
     """Drafts down to the narrowest window change no answer (32-bit); deeper ones are refused."""
