@@ -77,6 +77,9 @@ def _ctx_bucket(n: int) -> int:
 PROMPT_GRAPH_RULES = ((128 << 20, 256), (400 << 20, 128))      # (bytes of a layer at most, tokens at most)
 PROMPT_GRAPH_TIMES = 4
 PROMPT_GRAPHS = 8                                              # how many are kept at most
+# Trees of drafted tokens go by the same rules and the same sizes, with graphs of their own (a row of logits a node makes each larger); a drafting loop
+# runs little else, so a size comes back soon and is captured the third time.
+TREE_GRAPH_TIMES = 3
 
 
 def _prompt_graph_tokens(layer_bytes: int) -> int:
@@ -130,7 +133,7 @@ class Engine:
                  max_graphs: int = 8):
         """``max_graphs``: how many captured decode graphs are kept (one per batch bucket and context
         bucket, least recently used dropped first); each holds its own activations and logits.  As many graphs of short prompts, up to
-        ``PROMPT_GRAPHS`` and as the memory left over allows, are kept beside them."""
+        ``PROMPT_GRAPHS`` and as the memory left over allows, are kept beside them, and then as many of trees of drafted tokens."""
         self.model = model
         self.env = model.env
         self.device = model.env.device
@@ -149,7 +152,9 @@ class Engine:
         if self.use_graphs and self.env.act_dtype == torch.bfloat16 and all(plain_layer(b) for b in model.blocks):
             self._prompt_graph_tokens = _prompt_graph_tokens(max(b.weight_bytes() for b in model.blocks))
         self._one_kernel = decode_layers.fits(model)
+        self._spare_bytes = 0      # what the budget leaves beside everything that is kept
         self._prompt_sizes = GraphSizes(self._check_budget(max_tokens, max_slots))
+        self._tree_sizes = GraphSizes(self._tree_graphs_that_fit(), TREE_GRAPH_TIMES)
         self.cache = SequenceCache(
             model.cache_requirements(), model.reads_cache_of(), max_tokens, max_slots,
             min(model.spec.max_position, max_seq_len or model.spec.max_position), self.env.act_dtype,
@@ -216,7 +221,18 @@ class Engine:
         if not self._prompt_graph_tokens:
             return 0
         each = self.model.workspace_bytes(self._prompt_graph_tokens, min(_bucket(max_slots), self._prompt_graph_tokens))
-        return min(PROMPT_GRAPHS, self.max_graphs, (free - need - headroom) // each)
+        kept = min(PROMPT_GRAPHS, self.max_graphs, (free - need - headroom) // each)
+        self._spare_bytes = free - need - headroom - kept * each
+        return kept
+
+    def _tree_graphs_that_fit(self) -> int:
+        """How many graphs of trees of drafted tokens fit into what ``_check_budget`` left: a row of logits a node, and what attention over trees works in."""
+        if not self._prompt_graph_tokens or not self.model.takes_trees:
+            return 0
+        from .. import kernels
+        each = self.model.workspace_bytes(self._prompt_graph_tokens, self._prompt_graph_tokens) + max(
+            kernels.tree_work_bytes(b.mixer.nkv, b.mixer.hdp, self.device) for b in self.model.blocks)
+        return min(PROMPT_GRAPHS, self.max_graphs, self._spare_bytes // each)
 
     # ---- construction ----------------------------------------------------------------------------
     @staticmethod
@@ -423,14 +439,13 @@ class Engine:
         self.last_h2d_bytes = buf.h2d_bytes
         def batch(capturing=False):
             return self._batch(buf, t_pad, b_pad, w_pad, max_q, ctx_pad, is_decode, None if capturing else host, at_once, capturing)
-        first_plainly = is_decode or tree is not None
-        if g["graph"] is None and not first_plainly and not g["plain"]:
-            self._capture(g, batch(capturing=True))              # (a prompt of this size has run before)
+        if g["graph"] is None and not is_decode and not g["plain"]:
+            self._capture(g, batch(capturing=True))              # (a prompt, or trees, of this size have run before)
         if g["graph"] is None:
-            # First use of a bucket of single tokens or trees: run it plainly (this also loads every kernel), then
+            # First use of a decode bucket: run it plainly (this also loads every kernel), then
             # capture the same launches for the next time.  Capturing executes nothing.
             out = self.model.forward(batch(), self.cache)
-            if first_plainly and not g["plain"]:
+            if is_decode and not g["plain"]:
                 torch.cuda.current_stream().synchronize()
                 self._capture(g, batch(capturing=True))
                 self.graphs_captured += g["graph"] is not None

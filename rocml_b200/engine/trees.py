@@ -113,6 +113,7 @@ class TreeSteps:
 
     def _run(self, entries):
         """(logits of a piece's nodes, its buffers on the device, the nodes' depths)."""
+        from .engine import _bucket
         eng = self.engine
         slots, tokens = [e.slot for e in entries], [list(e.tokens) for e in entries]
         olds = [eng.cache.grow(e.slot, len(e.tokens)) for e in entries]
@@ -126,23 +127,27 @@ class TreeSteps:
         eng._device_tokens = None
         eng._replayed = False
         prof = _profiler.ACTIVE
-        # short steps are replayed from graphs where short prompts are
-        if prof is None and eng.use_graphs and T <= eng._prompt_graph_tokens:
-            from .engine import _bucket
-            t_pad, b_pad = _bucket(T, 16), _bucket(B)
-            pads = (t_pad, b_pad, t_pad, min(MAX_NODES, _bucket(max(q_lens), 16)), _bucket(max(kv_len), 1024), False)
-            logits = eng._run_graph(eng._tree_graphs, eng.max_graphs, pads, packed, host, T, pads, tree=tree)
-            return logits, eng._last_buffers, depths
-        from .engine import _bucket
+        pads = None
+        # short steps are replayed from graphs where short prompts are, if their sizes come back and there is memory for them
+        if prof is None and T <= eng._prompt_graph_tokens and eng._tree_sizes.kept:
+            t_pad = _bucket(T, 16)
+            pads = (t_pad, _bucket(B), t_pad, min(MAX_NODES, _bucket(max(q_lens), 16)), _bucket(max(kv_len), 1024), False)
+            due = eng._tree_sizes.due(pads, eng._tree_graphs)
+            eng._tree_sizes.note(pads)
+            if due:
+                logits = eng._run_graph(eng._tree_graphs, eng._tree_sizes.kept, pads, packed, host, T, pads, tree=tree)
+                return logits, eng._last_buffers, depths
         key = (_bucket(T, 64), _bucket(B, 8))
         if key not in self._buffers:
             self._buffers[key] = BatchBuffers(key[0], key[1], key[0], eng.device, trees=True)
         buf = self._buffers[key]
-        buf.fill(*packed, slots, pad_tokens=T, pad_seqs=B, pad_want=T, tree=tree)
+        # (padded as the graph will be: an answer does not depend on how often its size has come)
+        t_pad, b_pad, w_pad, max_q, max_kv, _ = pads or (T, B, T, max(q_lens), max(kv_len), False)
+        buf.fill(*packed, slots, pad_tokens=t_pad, pad_seqs=b_pad, pad_want=w_pad, tree=tree)
         eng.last_h2d_bytes = buf.h2d_bytes
-        batch = eng._batch(buf, T, B, T, max(q_lens), max(kv_len), False, host)
+        batch = eng._batch(buf, t_pad, b_pad, w_pad, max_q, max_kv, False, host)
         if prof is None:
-            return eng.model.forward(batch, eng.cache), buf, depths
+            return eng.model.forward(batch, eng.cache)[:T], buf, depths
         with prof.step("prefill", q_lens, kv_len):
             return eng.model.forward(batch, eng.cache), buf, depths
 

@@ -976,6 +976,13 @@ def _tree_plan(tensor_cores: bool, n_seqs: int, max_nodes: int, group: int, nkv:
     return rows_tile, shares, cluster, 0 if shares == 1 or cluster else 2 * shares * nkv * rows_tile * (hd + 2) + 4 * nkv * min(shares - 1, units)
 
 
+def tree_work_bytes(nkv: int, hd: int, device) -> int:
+    """The most work space that a call of attention_tree takes, whatever its sequences (``_tree_plan``; shares come two places each, nkv * shares of them)."""
+    blocks = _decode_slots(device) // 3 * 2
+    blocks = blocks if nkv <= blocks else 4 * blocks + nkv
+    return 4 * (2 * blocks * 128 * (hd + 2) + 4 * blocks)
+
+
 @_profiled(lambda a, facts: _attention_cost(a, facts))
 def attention_tree(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                    seq_slot: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor, visible: torch.Tensor, n_seqs: int, max_nodes: int,

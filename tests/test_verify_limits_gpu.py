@@ -11,6 +11,54 @@ from tiny_models import _dense, _latent, _layer, prompt, write_pipilix
 pytestmark = pytest.mark.gpu
 
 
+def least_memory(eng, max_tokens, max_slots, monkeypatch):
+    """The free memory with which an engine like this is just accepted, found through the refusals."""
+    from rocml_b200 import MemoryBudget
+    lo, hi = 0, 4 << 30
+    while hi - lo > 1:
+        mid = (lo + hi) // 2
+        monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a, m=mid: (m, 180 << 30))
+        try:
+            eng._check_budget(max_tokens, max_slots)
+            hi = mid
+        except MemoryBudget:
+            lo = mid
+    return hi
+
+
+def test_graphs_of_trees_take_only_memory_that_is_left(folders, monkeypatch):        # noqa: F811
+    """An engine that just fits keeps none; the graphs of short prompts come first, then as many of trees as fit, each with logits for all its nodes.
+    The answers are the same bits, and a size is captured only when it has come a few times."""
+    from rocml_b200 import Engine, StepEntry, TreeEntry
+    from rocml_b200.engine.engine import PROMPT_GRAPHS
+    vocab = vocab_of("D")
+    eng = Engine.from_folder(folders("D"), dtype="bfloat16", max_tokens=1024, max_slots=4)
+    model, tokens = eng.model, eng._prompt_graph_tokens
+    least = least_memory(eng, 1024, 4, monkeypatch)
+    prompts = PROMPT_GRAPHS * model.workspace_bytes(tokens, 4)
+    logits = tokens * vocab * 4
+    ids, rng = prompt(8, 50, vocab), random.Random(2)
+    trees = [random_tree(rng, n, vocab) for n in (9, 40, 100)]
+    answers = []
+    for spare in (0, prompts, prompts + logits, prompts + (4 << 30)):
+        monkeypatch.setattr(torch.cuda, "mem_get_info", lambda *a: (least + spare, 180 << 30))
+        eng = Engine(model, max_tokens=1024, max_slots=4)
+        slot = eng.new_sequence()
+        eng.step([StepEntry(slot, ids)])
+        got = []
+        for turn in range(6):
+            for t, p in trees:
+                got.append(eng.tree_logits([TreeEntry(slot, t, p)]).clone())
+            if turn == 0:
+                assert not eng._tree_graphs
+        assert all(torch.equal(a, b) for a, b in zip(got, got[3:]))
+        assert len(eng._tree_graphs) == (3 if spare > prompts + logits else 0), spare
+        answers.append(got[:3])
+    for a in answers:
+        for x, y in zip(a, answers[-1]):
+            assert rel_err(x, y) < 2 * TOL["bfloat16"]
+
+
 @pytest.mark.parametrize("name,step_tokens", [("A", 4), ("A", 1), ("B", 20), ("C", 4096), ("E", 7), ("PA", 4096), ("PB", 12), ("PC", 4096)])
 def test_drafts_that_an_engine_cannot_take_are_cut(folders, name, step_tokens):        # noqa: F811
     """More guesses than a step holds, deeper ones than a window: the answers are the ordinary ones (32-bit), also where no guess is left."""
