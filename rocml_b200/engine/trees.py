@@ -179,59 +179,62 @@ class TreeSteps:
         for e, p, r in zip(entries, params, rngs):
             if not p.is_greedy and r is None:
                 raise RocmlError(f"slot {e.slot}: sampling needs a random stream")
-        results, at = [], 0
         with torch.cuda.device(self.engine.device):
-            for piece in self._pieces(entries):
-                k = len(piece)
-                results += self._verify_piece(piece, params[at:at + k], rngs[at:at + k], histories[at:at + k])
-                at += k
-        return results
+            try:
+                # Everything that can fail comes before any sequence grows or stream moves on: a path's keys and values are moved to places behind its
+                # sequence's length, where nothing reads them yet.
+                settled, at = [], 0
+                for piece in self._pieces(entries):
+                    k = len(piece)
+                    settled += self._settle_piece(piece, params[at:at + k], rngs[at:at + k], histories[at:at + k])
+                    at += k
+                results = []
+                for e, p, r, (way, last) in zip(entries, params, rngs, settled):
+                    self.engine.cache.commit(e.slot, len(way))
+                    if not p.is_greedy:
+                        for _ in way:
+                            r.next_f32()
+                    results.append([int(e.tokens[i]) for i in way[1:]] + [last])
+                return results
+            finally:
+                for e in entries:
+                    self.engine.cache.trim(e.slot)
 
-    def _verify_piece(self, entries, params, rngs, histories):
+    def _settle_piece(self, entries, params, rngs, histories):
+        """The confirmed path of every tree, and the token sampled at its end."""
         eng = self.engine
-        try:
-            logits, buf, depths = self._run(entries)
-            if self._sampler is None:
-                from ..sampling import Sampler
-                self._sampler = Sampler(eng.device, max_batch=self.max_nodes)
-            row_params, row_rngs, row_histories, row = [], [], [], 0
-            for e, p, r, h in zip(entries, params, rngs, histories):
-                m = len(e.tokens)
-                depth = depths[row:row + m]
-                ahead = copy.copy(r) if not p.is_greedy else None       # the stream itself moves on once it is known by how much
-                draws = [_Drawn(ahead.next_f32()) for _ in range(max(depth) + 1)] if ahead is not None else None
-                row_params += [p] * m
-                row_rngs += [None] * m if draws is None else [draws[d] for d in depth]
-                if p.repeat_penalty is None:
-                    row_histories += [h] * m
-                else:
-                    paths = [list(h)]
-                    for i in range(1, m):
-                        paths.append(paths[e.parents[i]] + [int(e.tokens[i])])
-                    row_histories += paths
-                row += m
-            handle = self._sampler.launch(logits, row_params, row_rngs, row_histories, status=kernels.status_word(eng.device))
-            B, most = len(entries), max(len(e.tokens) for e in entries)
-            out = torch.empty(B * (most + 2), dtype=torch.int32, device=eng.device)
-            path, counts, nxt = out[:B * most].view(B, most), out[B * most:B * (most + 1)], out[B * (most + 1):]
-            tree = buf.tree(row, most)
-            settle = lambda **cache: kernels.tree_accept(buf.token_ids, tree.parents, tree.visible, handle.device_tokens, buf.cu_q, B, path, counts,
-                                                         nxt, **cache)
-            if not eng.cache.kv_groups:
-                settle()
-            for g in eng.cache.kv_groups:
-                settle(seq_slot=buf.seq_slot, kv_len=buf.kv_len, block_table=g.table, k=g.k, v=g.v)
-            got = out.cpu()                                  # (this waits for the step)
-            kernels.raise_for_status(int(handle.host_status[0]))
-            paths, counts, nxt = got[:B * most].view(B, most).tolist(), got[B * most:B * (most + 1)].tolist(), got[B * (most + 1):].tolist()
-            results = []
-            for e, p, r, way, count, last in zip(entries, params, rngs, paths, counts, nxt):
-                eng.cache.commit(e.slot, count)
-                if not p.is_greedy:
-                    for _ in range(count):
-                        r.next_f32()
-                results.append([int(e.tokens[i]) for i in way[1:count]] + [last])
-            return results
-        finally:
-            for e in entries:
-                eng.cache.trim(e.slot)
+        logits, buf, depths = self._run(entries)
+        if self._sampler is None:
+            from ..sampling import Sampler
+            self._sampler = Sampler(eng.device, max_batch=self.max_nodes)
+        row_params, row_rngs, row_histories, row = [], [], [], 0
+        for e, p, r, h in zip(entries, params, rngs, histories):
+            m = len(e.tokens)
+            depth = depths[row:row + m]
+            ahead = copy.copy(r) if not p.is_greedy else None       # the stream itself moves on once it is known by how much
+            draws = [_Drawn(ahead.next_f32()) for _ in range(max(depth) + 1)] if ahead is not None else None
+            row_params += [p] * m
+            row_rngs += [None] * m if draws is None else [draws[d] for d in depth]
+            if p.repeat_penalty is None:
+                row_histories += [h] * m
+            else:
+                paths = [list(h)]
+                for i in range(1, m):
+                    paths.append(paths[e.parents[i]] + [int(e.tokens[i])])
+                row_histories += paths
+            row += m
+        handle = self._sampler.launch(logits, row_params, row_rngs, row_histories, status=kernels.status_word(eng.device))
+        B, most = len(entries), max(len(e.tokens) for e in entries)
+        out = torch.empty(B * (most + 2), dtype=torch.int32, device=eng.device)
+        path, counts, nxt = out[:B * most].view(B, most), out[B * most:B * (most + 1)], out[B * (most + 1):]
+        tree = buf.tree(row, most)
+        settle = lambda **cache: kernels.tree_accept(buf.token_ids, tree.parents, tree.visible, handle.device_tokens, buf.cu_q, B, path, counts,
+                                                     nxt, **cache)
+        if not eng.cache.kv_groups:
+            settle()
+        for g in eng.cache.kv_groups:
+            settle(seq_slot=buf.seq_slot, kv_len=buf.kv_len, block_table=g.table, k=g.k, v=g.v)
+        got = out.cpu()                                  # (this waits for the step)
+        kernels.raise_for_status(int(handle.host_status[0]))
+        paths, counts, nxt = got[:B * most].view(B, most).tolist(), got[B * most:B * (most + 1)].tolist(), got[B * (most + 1):].tolist()
+        return [(way[:count], last) for way, count, last in zip(paths, counts, nxt)]

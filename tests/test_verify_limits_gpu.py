@@ -59,6 +59,46 @@ def test_graphs_of_trees_take_only_memory_that_is_left(folders, monkeypatch):   
             assert rel_err(x, y) < 2 * TOL["bfloat16"]
 
 
+def test_verify_in_pieces_is_one_act(folders, monkeypatch):        # noqa: F811
+    """If a later piece fails, no sequence has grown, no stream has moved on and no page is lost; the same call then gives what it would have given."""
+    from rocml_b200 import Engine, SamplingParams, StepEntry, TreeEntry
+    from rocml_b200.sampling import XorShift64Star
+    vocab = vocab_of("D")
+    rng = random.Random(12)
+    ctx = [prompt(70 + n, n, vocab) for n in (130, 20, 64, 100)]
+    trees = [random_tree(rng, n, vocab) for n in (200, 190, 180, 250)]
+    params = [SamplingParams(), SamplingParams(0.8, 40, seed=3), SamplingParams(0.9, 30, None, seed=9, repeat_penalty=1.3), SamplingParams(1.0, seed=4)]
+
+    def start():
+        eng = Engine.from_folder(folders("D"), dtype="float32", max_tokens=64 * 40, max_slots=8)
+        slots = [eng.new_sequence() for _ in ctx]
+        eng.step([StepEntry(s, c) for s, c in zip(slots, ctx)])
+        return eng, slots, [TreeEntry(s, t, p) for s, (t, p) in zip(slots, trees)], [XorShift64Star(5 + i) for i in range(4)]
+    eng, slots, entries, streams = start()
+    histories = [c + [t[0]] for c, (t, _) in zip(ctx, trees)]
+    want = eng.verify(entries, params, streams, histories)
+    want_lengths, want_next = [eng.length(s) for s in slots], [s.next_f32() for s in streams]
+    eng, slots, entries, streams = start()
+    run, calls = eng._tree_steps()._run, []
+
+    def failing(piece):
+        calls.append(len(piece))
+        if len(calls) > 1:
+            raise RuntimeError("the second piece")
+        return run(piece)
+    free = [g.pool.n_free for g in eng.cache.kv_groups]
+    with monkeypatch.context() as m:
+        m.setattr(eng._tree_steps(), "_run", failing)
+        with pytest.raises(RuntimeError, match="second piece"):
+            eng.verify(entries, params, streams, histories)
+    assert len(calls) == 2 and [eng.length(s) for s in slots] == [len(c) for c in ctx]
+    eng.cache.check_invariants()
+    assert [g.pool.n_free for g in eng.cache.kv_groups] == free
+    assert eng.verify(entries, params, streams, histories) == want
+    assert [eng.length(s) for s in slots] == want_lengths and [s.next_f32() for s in streams] == want_next
+    eng.cache.check_invariants()
+
+
 @pytest.mark.parametrize("name,step_tokens", [("A", 4), ("A", 1), ("B", 20), ("C", 4096), ("E", 7), ("PA", 4096), ("PB", 12), ("PC", 4096)])
 def test_drafts_that_an_engine_cannot_take_are_cut(folders, name, step_tokens):        # noqa: F811
     """More guesses than a step holds, deeper ones than a window: the answers are the ordinary ones (32-bit), also where no guess is left."""
