@@ -8,12 +8,14 @@ import torch
 from ..errors import RocmlError
 from ..sampling.scorer import Scorer, TokenScore, check_top
 
-# Rows of logits that are scored at a time: 311 MB of them at a vocabulary of 151,936, inside the head room of the engine's memory budget.
+# Rows of logits that are scored at a time, and their bytes at most: less than half of the head room of the engine's memory budget (512 rows are 297 MiB at a
+# vocabulary of 151,936; a vocabulary of 262,144 takes 320 rows).  One piece's are held at a time.
 SCORE_ROWS = 512
+SCORE_BYTES = 320 << 20
 
 
 def score(engine, sequences: Sequence[Sequence[int]], top: int = 0) -> List[List[TokenScore]]:
-    """See ``Engine.score``.  Sequence after sequence, in pieces of ``SCORE_ROWS`` tokens; each takes a slot and gives it back."""
+    """See ``Engine.score``.  Sequence after sequence, in pieces of ``SCORE_ROWS`` tokens at most; each takes a slot and gives it back."""
     from .engine import StepEntry
     top = check_top(top, engine.model.vocab)
     sequences = [[int(t) for t in s] for s in sequences]
@@ -25,7 +27,7 @@ def score(engine, sequences: Sequence[Sequence[int]], top: int = 0) -> List[List
         bad = [t for t in s if not 0 <= t < engine.model.vocab]
         if bad:
             raise RocmlError(f"sequence {i}: token id {bad[0]} is outside the vocabulary of {engine.model.vocab}")
-    rows = min(SCORE_ROWS, engine.max_step_tokens)
+    rows = min(SCORE_ROWS, max(1, SCORE_BYTES // (4 * engine.model.vocab)), engine.max_step_tokens)
     scorer = Scorer(engine.device, max_batch=rows, depth=2)
     out = []
     for s in sequences:
@@ -39,6 +41,7 @@ def score(engine, sequences: Sequence[Sequence[int]], top: int = 0) -> List[List
                 with torch.cuda.device(engine.device):
                     after = torch.tensor(s[a + 1:a + 1 + len(piece)], dtype=torch.int32).to(engine.device)
                     pending = scorer.launch(logits, after, top)
+                del logits                       # (before the next piece's are made; the memory is used again in the stream's order)
                 if waiting is not None:
                     found += scorer.collect(waiting)
                 waiting = pending

@@ -89,6 +89,43 @@ def test_a_step_takes_no_more_sequences_than_its_kernels():
     assert all(sum(len(e.tokens) for e in p) <= 4096 for p in pieces) and len(pieces) == 3
 
 
+@pytest.mark.parametrize("vocab", [300, 151936, 262144, 2 ** 27])
+def test_scoring_holds_the_logits_of_one_piece(vocab, monkeypatch):
+    """A piece's logits go before the next one's come, and are no more than 320 MiB (one row at least)."""
+    from rocml_b200.engine import scoring
+    from rocml_b200.sampling import TokenScore
+    alive, rows = [], []
+
+    def step(entries):
+        assert not any(r() is not None for r in alive)
+        n = len(entries[0].tokens)
+        rows.append(n)
+        logits = torch.zeros((n, 1))
+        alive.append(weakref.ref(logits))
+        return logits
+
+    class Scorer:
+        def __init__(self, device, max_batch, depth):
+            self.max_batch = max_batch
+
+        def launch(self, logits, tokens, top):
+            assert logits.shape[0] == tokens.numel() <= self.max_batch
+            return tokens.tolist()
+
+        @staticmethod
+        def collect(tokens):
+            return [TokenScore(t, 0.0, 0.0, []) for t in tokens]
+    monkeypatch.setattr(scoring, "Scorer", Scorer)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(kernels, "check_status", lambda d: None)
+    engine = SimpleNamespace(model=SimpleNamespace(vocab=vocab), max_seq_len=4000, max_step_tokens=4096, device=torch.device("cpu"), step=step,
+                             new_sequence=lambda: 0, release=lambda s: None)
+    text = [i % 299 for i in range(1100 if vocab < 2 ** 27 else 5)]
+    got = scoring.score(engine, [text, text[:2]])
+    assert [[s.token for s in g] for g in got] == [text[1:], text[1:2]]
+    assert max(rows) == max(1, min(512, (320 << 20) // (4 * vocab)))
+
+
 class _OnAnotherDevice(torch.Tensor):
     def get_device(self):
         return 5
