@@ -104,3 +104,35 @@ def test_as_many_kept_places_as_an_integer_holds(dtype, hd):
     for keep in (2 ** 31 - 1, 2 ** 31 - 64, 2 ** 20):
         check(t, dtype, call(t, window=5, keep=keep), window=5, keep=keep)
     check(t, dtype, call(t, window=2 ** 31 - 1, keep=2 ** 31 - 1))
+
+
+@pytest.mark.parametrize("sizes", [[(70, 9), (0, 3)], [(1500, 17), (64, 40)]])
+@pytest.mark.parametrize("dtype,nq,hd", [(torch.float32, 16, 32), (torch.bfloat16, 9, 64), (torch.bfloat16, 32, 128), (torch.bfloat16, 17, 256), (torch.bfloat16, 20, 512)])
+def test_keys_and_values_in_one_tensor(sizes, dtype, nq, hd):
+    """A latent that serves as both, read by many heads: attention over it, and the confirmed path's rows moved once."""
+    from rocml_b200 import kernels
+    t = Trees(nq, sizes, nq, 1, hd, dtype, layers=2)
+    t.v = t.k
+    d = t.ints(DEV)
+    both = t.k.to(DEV)
+    q = t.q.to(DEV)
+    out = torch.full_like(q, 7.0)
+    kernels.attention_tree(q, out, both[0], both[0], d["block_table"], d["seq_slot"], d["cu_q"], d["kv_len"], d["visible"], 2, max(n for _, n in sizes), nq, 1,
+                           hd, hd ** -0.5, max_kv_len=max(c + n for c, n in sizes), positions=t.positions.to(DEV), window=200)
+    kernels.check_status(DEV)
+    check(t, dtype, out, window=200)
+    tokens = [list(range(n)) for _, n in sizes]
+    sampled = [[max([j for j, up in enumerate(p) if up == i], default=0) for i in range(len(p))] for p in t.parents]       # (the last child)
+    want, i32 = t.k.clone(), lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    moved = 0
+    for b, (c, n) in enumerate(sizes):
+        for depth, node in enumerate(plain_tree.accept(t.parents[b], tokens[b], sampled[b])[0]):
+            (p, i), (sp, si) = t.place(b, c + depth), t.place(b, c + node)
+            want[:, p, :, i] = t.k[:, sp, :, si]
+            moved += node > depth
+    assert moved
+    path = torch.zeros((2, max(n for _, n in sizes)), dtype=torch.int32, device=DEV)
+    flat = lambda x: i32([y for s in x for y in s])
+    kernels.tree_accept(flat(tokens), flat(t.parents), d["visible"], flat(sampled), d["cu_q"], 2, path, i32([0, 0]), i32([0, 0]), seq_slot=d["seq_slot"],
+                        kv_len=d["kv_len"], block_table=d["block_table"], k=both, v=both)
+    assert torch.equal(both.cpu(), want)

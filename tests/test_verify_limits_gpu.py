@@ -125,6 +125,47 @@ def test_drafts_that_an_engine_cannot_take_are_cut(folders, name, step_tokens): 
     assert eng.cache.slots.n_held == 0
 
 
+@pytest.mark.parametrize("heads,rank", [(16, 64), (20, 128), (8, 48)])
+def test_trees_over_latents_in_bfloat16(tmp_path, heads, rank):
+    """Layers whose cached rows are keys and values at once: every node's logits against its path as an ordinary prompt, and greedy verifying against the
+    most likely tokens."""
+    from rocml_b200 import Engine, SamplingParams, StepEntry, TreeEntry
+    config = {"architecture": "Pipilix", "vocab": 333, "width": 128, "embedding": {"scale": 1.0}, "norm": {"eps": 1e-5}, "logit_scale": 1.0,
+              "layers": [_layer(_latent(heads, 32, 32, rank, 200, 0.18), _dense(160)), _layer(_latent(heads, 16, 24, rank, 300, 0.25), _dense(96))]}
+    write_pipilix(str(tmp_path), config, seed=6)
+    eng = Engine.from_folder(str(tmp_path), dtype="bfloat16", max_tokens=1024, max_slots=3)
+    rng = random.Random(8)
+    ctx = [prompt(n, n, 333) for n in (64, 150)]
+    slots = [eng.new_sequence() for _ in ctx]
+    eng.step([StepEntry(s, c) for s, c in zip(slots, ctx)])
+    trees = [random_tree(rng, n, 333) for n in (12, 5)]
+    entries = [TreeEntry(s, t, p) for s, (t, p) in zip(slots, trees)]
+    logits, row = eng.tree_logits(entries).clone(), 0
+    for c, (tokens, parents) in zip(ctx, trees):
+        for i in range(len(tokens)):
+            way = [tokens[j] for j in path_to(parents, i)]
+            slot = eng.new_sequence()
+            want = eng.step([StepEntry(slot, c + way, [len(c) + len(way) - 1])])
+            eng.release(slot)
+            assert rel_err(logits[row:row + 1], want) < 2 * TOL["bfloat16"], i
+            row += 1
+    # trees that hold the most likely token behind the root, after a wrong one
+    best = [int(logits[0].argmax()), int(logits[12].argmax())]
+    entries = [TreeEntry(s, [t[0], (b + 1) % 333, b], [-1, 0, 0]) for s, (t, _), b in zip(slots, trees, best)]
+    lone = eng.tree_logits(entries).clone()
+    got = eng.verify(entries, [SamplingParams()] * 2)
+    for i, (c, (t, _), b, g) in enumerate(zip(ctx, trees, best, got)):
+        if int(lone[3 * i].argmax()) != b:             # (a near tie fell differently in the other tree)
+            continue
+        assert g[0] == b and len(g) == 2 and eng.length(slots[i]) == len(c) + 2
+        # the row that was moved is read again: as a prompt
+        again = eng.step([StepEntry(slots[i], [g[1]], [0])]).clone()
+        slot = eng.new_sequence()
+        want = eng.step([StepEntry(slot, c + [t[0], b, g[1]], [len(c) + 2])])
+        eng.release(slot)
+        assert rel_err(again, want) < 2 * TOL["bfloat16"]
+
+
 @pytest.mark.parametrize("windows", [(50, 7), (9, 50), (None, 12)])
 def test_layers_that_read_anothers_cache_through_another_window(tmp_path, windows):
     """Drafts down to the narrowest window change no answer (32-bit); deeper ones are refused."""
