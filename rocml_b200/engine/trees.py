@@ -11,6 +11,7 @@ token would have used, and the sequence's random stream moves on by as many draw
 from __future__ import annotations
 
 import copy
+import weakref
 from dataclasses import dataclass
 from typing import List, Optional, Sequence
 
@@ -74,7 +75,8 @@ class TreeSteps:
     def __init__(self, engine):
         if not engine.model.takes_trees:
             raise ConfigError("this model keeps more than keys and values a sequence, or masks that have no form for trees of drafted tokens")
-        self.engine = engine
+        # (not a reference that keeps it: an engine that is no longer held gives its memory and its graphs back at once)
+        self.engine = weakref.proxy(engine)
         # (a step's logits, one row a node, stay within the head room of the engine's memory budget)
         self.max_nodes = min(engine.max_step_tokens, max(2 * MAX_NODES, engine.cache.max_slots))
         # A node sees all its ancestors: they must lie in every layer's window (its own, whatever the cache keeps for another layer that reads it).

@@ -13,6 +13,10 @@ from rocml_b200.cache import SequenceCache
 from rocml_b200.errors import KernelError, RocmlError
 
 
+class Parts(SimpleNamespace):
+    """What of an engine is asked for."""
+
+
 @pytest.mark.parametrize("keeper,reader,deepest", [(50, 7, 7), (9, 50, 9), (None, 8, 8), (12, None, 12), (None, None, 256)])
 def test_the_narrowest_window_of_any_layer_bounds_a_tree(keeper, reader, deepest):
     """Also where the cache keeps more, for another layer that reads it."""
@@ -25,7 +29,8 @@ def test_the_narrowest_window_of_any_layer_bounds_a_tree(keeper, reader, deepest
            "layers": [_kdiff(4, 2, 12, 20, 0.5, 0.3, _KA_ROT, 96, size=keeper), _kdiff(4, 2, 12, 20, 0.7, 0.5, _KA_ROT, 48, size=reader, kv_from=0)]}
     model = Model(config_from_dict(cfg).to_model_spec(), BuildEnv(torch.device("cpu"), torch.float32))
     cache = SequenceCache(model.cache_requirements(), model.reads_cache_of(), 1024, 2, 1024, torch.float32, torch.device("cpu"), 512)
-    steps = TreeSteps(SimpleNamespace(model=model, cache=cache, max_step_tokens=512))
+    engine = Parts(model=model, cache=cache, max_step_tokens=512)
+    steps = TreeSteps(engine)
     slot = cache.alloc_slot()
     chain = lambda n: TreeEntry(slot, [1] * n, list(range(-1, n - 1)))
     assert steps._check([chain(deepest)])

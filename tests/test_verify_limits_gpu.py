@@ -189,3 +189,37 @@ def test_layers_that_read_anothers_cache_through_another_window(tmp_path, window
         assert rel_err(g[None], want) < 2 * TOL["float32"]
     with pytest.raises(RocmlError, match="window"):
         eng.tree_logits([TreeEntry(slot, way + [1], list(range(-1, deepest)))])
+
+
+def test_an_engine_that_verified_is_gone_when_it_is_dropped(folders):        # noqa: F811
+    """Its memory with it, without waiting for the collector of cycles (which may come while another engine captures a graph, and graphs that go then spoil
+    the capture)."""
+    import gc
+    import weakref
+    from rocml_b200 import Engine, PromptLookup
+    vocab = vocab_of("D")
+    torch.cuda.synchronize()
+    gc.collect()
+    gc.disable()
+    try:
+        before = torch.cuda.memory_allocated()
+        for use in ("plain", "trees", "drafts", "scores"):
+            eng = Engine.from_folder(folders("D"), dtype="bfloat16", max_tokens=1024, max_slots=4)
+            assert torch.cuda.memory_allocated() > before
+            if use == "plain":
+                eng.generate([prompt(1, 20, vocab)], max_new_tokens=5)
+            elif use == "trees":
+                from rocml_b200 import TreeEntry
+                slot = eng.new_sequence()
+                for _ in range(4):
+                    eng.tree_logits([TreeEntry(slot, [1, 2, 3], [-1, 0, 0])])
+                assert eng._tree_graphs
+            elif use == "drafts":
+                eng.generate([[1, 2, 3] * 5], max_new_tokens=30, drafter=PromptLookup())
+            else:
+                eng.score([prompt(1, 20, vocab)], top=2)
+            gone = weakref.ref(eng)
+            del eng
+            assert gone() is None, use
+    finally:
+        gc.enable()
