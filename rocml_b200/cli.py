@@ -264,7 +264,7 @@ def main(argv=None) -> int:
     g.add_argument("--logprobs", type=int, default=None, metavar="K",
                    help="score every token: its log probability, the entropy and K alternatives (0 to 32)")
     g.add_argument("--draft", type=int, default=0, metavar="N",
-                   help="verify drafts of up to N tokens that followed the text's last tokens before (the answer is the same)")
+                   help="verify drafts of up to N tokens that followed the text's last tokens before (the same answer, but for near ties in bfloat16)")
     _profile_args(g)
     g.set_defaults(fn=cmd_generate)
 

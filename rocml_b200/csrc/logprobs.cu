@@ -13,7 +13,7 @@
 //
 // A row is read by one block or by the blocks of a cluster, which meet in the first one's shared memory.
 //
-// Memory bounds it where there are rows enough (2,047 rows of 151,936: 192 us, 6.5 TB/s); one row with 20 alternatives takes 7.8 us, 4.6 of them without.
+// Memory bounds it where there are rows enough (2,047 rows of 151,936: 192 us, 6.5 TB/s); one row with 20 alternatives takes 7.8 us, 4.7 without.
 // The ones counted apart cost 1 % of 32-bit rows; packed arithmetic and packed maxima give it back, and 5 % more, to bf16 ones, which the arithmetic bounds.
 #include "common.cuh"
 #include "api.h"

@@ -2,7 +2,13 @@
 
 A *drafter* is called with a sequence's tokens so far (prompt and answer) and returns (tokens, parents): guesses at what follows,
 ``parents[i]`` the earlier guess that guess i follows, -1 where it follows the sequence's last token.  Guesses cost a step's extra rows; those that the
-model would have sampled itself save a step each.  The answers are those of ordinary generation with the same parameters.
+model would have sampled itself save a step each.  The answers are those of ordinary generation with the same parameters, but for near ties:
+verifying rounds otherwise than a step of single tokens (other kernels, other orders of sums), so where two tokens are equally likely within rounding, or a draw falls
+that close to a border, the other one may come.  In bfloat16 that happens; in 32 bits hardly ever.
+
+What a draft has to bring.  A verifying step costs more than a decode step (contexts of 1,000 tokens, trees of 8 nodes: 1.3 times at 8b sizes and 1.8 at 0.6b, eight
+sequences 1.4 and 2.0), also where there is no guess, and the drafter's time on the host comes on top: ``PromptLookup`` looks through the whole text, 0.3 ms a
+sequence at 1,000 tokens without a match, 8 ms at 30,000.
 """
 from __future__ import annotations
 
@@ -80,7 +86,7 @@ def _entry(slot: int, history: Sequence[int], drafter: Drafter, room: int, nodes
 
 def generate_drafted(engine, requests: Sequence[Request], drafter: Drafter, default_stop: Iterable[int] = (), max_batch: int = 64,
                      on_token: Optional[Callable[[int, int], bool]] = None, stats: Optional[GenerateStats] = None) -> List[Completion]:
-    """``generate`` with drafts: the same requests, the same answers."""
+    """``generate`` with drafts: the same requests, and the same answers but for near ties (see above)."""
     stats = stats if stats is not None else GenerateStats()
     default_stop = set(default_stop)
     limit = engine.max_seq_len

@@ -512,8 +512,8 @@ class Engine:
         an entry; a sequence's nodes of one depth share the draw that the ordinary loop would have used there); a child with that token
         is confirmed, and so on down.  Each sequence becomes longer by its first node and the confirmed ones; what comes back, an entry a
         list, are the confirmed children's tokens and the token sampled after the last of them, which the sequence does not hold yet: the
-        tokens that as many ordinary steps would have sampled.  ``histories`` (an entry: prompt and tokens so far, the first node's
-        included) is read for repeat penalties only."""
+        tokens that as many ordinary steps would have sampled, near ties in bfloat16 aside.  It is one act: if it fails, no sequence has grown.
+        ``histories`` (an entry: prompt and tokens so far, the first node's included) is read for repeat penalties only."""
         return self._tree_steps().verify(entries, params, rngs, histories)
 
     def score(self, sequences, top: int = 0):
@@ -592,7 +592,7 @@ class Engine:
         """Generate for a list of prompts (token id lists).  Returns a list of Completion.
         ``sampling`` is one SamplingParams for all or a list; stop tokens default to the model's.  ``logprobs``: every token comes with
         its log probability and so many alternatives (0 to 32).  ``drafter``: drafts of the tokens that may follow, verified several at a
-        time (``engine.drafting``); the tokens are the same without it."""
+        time (``engine.drafting``); the tokens are the same without it, but for near ties in bfloat16."""
         from ..sampling import SamplingParams
         from .generate import Request, generate
         if sampling is None:

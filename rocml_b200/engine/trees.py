@@ -5,8 +5,9 @@ them: their keys and values go behind the context in the order of the nodes, eac
 and sees the context and its ancestors.  ``verify`` then samples at every node, and one kernel finds the path that the samples confirm and moves its keys
 and values to the places where ordinary steps would have left them; the pages behind it are given back.
 
-The tokens are those of ordinary generation: a sequence's nodes of one depth share one draw, the one that the step of that
-token would have used, and the sequence's random stream moves on by as many draws as tokens were taken.
+The tokens are those of ordinary generation (but for near ties, which other kernels may round the other way): a sequence's nodes of one
+depth share one draw, the one that the step of that token would have used, and the sequence's random stream moves on by as many draws as
+tokens were taken.
 """
 from __future__ import annotations
 

@@ -1090,7 +1090,7 @@ LOGPROBS_MAX_TOP = 32
 @functools.lru_cache(maxsize=4096)
 def logprob_blocks(rows: int, vocab: int, device=0) -> int:
     """Blocks a row of token_logprobs: a power of two that about fills the device once, none with less than 2,048 logits; up to eight, which any
-    cluster may have, and sixteen for a few rows only (151,936 logits, 20 alternatives: one row 7.6 us with sixteen, 8.1 with eight, 32 rows 18 and
+    cluster may have, and sixteen for a few rows only (151,936 logits, 20 alternatives: one row 7.8 us with sixteen, 8.3 with eight, 32 rows 18 and
     13; 148 rows 31 with four, which would just fit, 24 with two)."""
     slots = 7 * _decode_slots(device) // 6             # seven eighths of four blocks a multiprocessor
     most = 16 if rows <= 8 else 8
