@@ -13,6 +13,7 @@ a chunk of one prompt: chunk_forward.rs:62-189; the chunk loop: :33-53) and no b
 """
 from __future__ import annotations
 
+import gc
 from collections import OrderedDict
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
@@ -468,6 +469,9 @@ class Engine:
             # (graphs share their memory, as no two run side by side; it goes with the last of them)
             pool = next((x["graph"].pool() for t in (self._graphs, self._prompt_graphs, self._tree_graphs) for x in t.values() if x["graph"] is not None), None)
             graph = torch.cuda.CUDAGraph()
+            # (an engine in a cycle of references that the collector found meanwhile would take its graphs with it, which spoils a capture)
+            collects = gc.isenabled()
+            gc.disable()
             try:
                 with torch.cuda.stream(self._capture_stream):
                     # (only this thread's calls are watched: others may allocate meanwhile)
@@ -482,6 +486,8 @@ class Engine:
                 if "out of memory" not in str(e):
                     raise
             finally:
+                if collects:
+                    gc.enable()
                 kernels.launch_count = before      # captured, not launched
             logits = None
             graph.reset()

@@ -223,3 +223,32 @@ def test_an_engine_that_verified_is_gone_when_it_is_dropped(folders):        # n
             assert gone() is None, use
     finally:
         gc.enable()
+
+
+def test_a_capture_is_not_spoiled_by_graphs_that_go(folders, monkeypatch):        # noqa: F811
+    """An engine in a cycle of references, found by the collector while another captures: its graphs go after the capture."""
+    import gc
+    from rocml_b200 import Engine, StepEntry
+    vocab = vocab_of("D")
+
+    def steps(eng):
+        slot = eng.new_sequence()
+        eng.step([StepEntry(slot, prompt(1, 20, vocab))])
+        return torch.cat([eng.step([StepEntry(slot, [t], [0])]).clone() for t in (3, 4, 5)])
+    old = Engine.from_folder(folders("D"), dtype="bfloat16", max_tokens=1024, max_slots=4)
+    want = steps(old)
+    old.itself, held = old, [old]
+    del old
+    eng = Engine.from_folder(folders("D"), dtype="bfloat16", max_tokens=1024, max_slots=4)
+    forward, captured = eng.model.forward, []
+
+    def drops(batch, cache):
+        if batch.capturing:
+            captured.append(len(held))
+            held.clear()
+            if gc.isenabled():                         # (the collector's turn, which comes whenever it is allowed to)
+                gc.collect()
+        return forward(batch, cache)
+    monkeypatch.setattr(eng.model, "forward", drops)
+    assert torch.equal(steps(eng), want)
+    assert captured == [1] and gc.isenabled() and eng.graphs_captured == 1
