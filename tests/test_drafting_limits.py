@@ -140,3 +140,16 @@ def test_a_sink_on_another_device_is_refused():
     from test_tree import _attention
     with pytest.raises(KernelError, match="one device"):
         _attention(sink=torch.zeros(8).as_subclass(_OnAnotherDevice))
+
+
+@pytest.mark.parametrize("hd", [16, 64, 80, 128, 256, 512])
+@pytest.mark.parametrize("group,nkv", [(1, 1), (4, 8), (7, 3), (128, 1), (2, 400)])
+def test_no_call_works_in_more_than_the_budget_counts(hd, group, nkv, monkeypatch):
+    monkeypatch.setattr(kernels, "_decode_slots", lambda device: 444)
+    most = kernels.tree_work_bytes(nkv, hd, 0)
+    for tensor_cores in {False, hd in (64, 128, 256)}:
+        for n_seqs in (1, 2, 5, 16, 33, 37, 256):
+            for nodes in (1, 9, 33, 256):
+                for pages in (1, 2, 7, 16, 64, 3000):
+                    plan = kernels._tree_plan.__wrapped__(tensor_cores, n_seqs, nodes, group, nkv, hd, pages, 0)
+                    assert 4 * plan[3] <= most
